@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define GSCAN_ABI_VERSION 14
+#define GSCAN_ABI_VERSION 15
 #define GSCAN_MAX_ENC_LAYERS 4
 
 /* Problem dimensions (names follow the reference's flags, seq2seq/__main__.py:21-102).
@@ -321,6 +321,83 @@ int gscan_early_gradients_wait(void *stream);
  * all-reduces only the rest on its own stream.  comm = NULL clears the registration (do so before gscan_comm_destroy).
  * Use a communicator of its own for this (not the one the late group travels on). */
 int gscan_comm_set_early_allreduce(void *comm, float *buf, size_t n);
+
+/* ---- operators over rows of logits (ABI 15; NOT in the reference): any vocabulary, float32 / bfloat16 / float16 ---- */
+#define GSCAN_F32 0
+#define GSCAN_BF16 1
+#define GSCAN_F16 2
+#define GSCAN_MAX_TOP 256      /* entries per row of a selection, of a teacher */
+#define GSCAN_MAX_BEAMS 64
+
+/* Rows of V adjacent words: row (o, i), 0 <= o < outer, 0 <= i < inner, begins at element o * stride_outer + i * stride_inner
+ * of `data`.  A row may begin at any element.  1 <= outer * inner <= 2^24, V <= 2^30. */
+typedef struct gscan_rows {
+    const void *data;
+    int32_t type;              /* GSCAN_F32, GSCAN_BF16, GSCAN_F16                  */
+    int32_t V;
+    int64_t outer, inner, stride_outer, stride_inner;
+} gscan_rows;
+
+/* The K best words of every row, best first (value descending, index ascending among equals; a NaN counts as -inf and is
+ * returned as -inf): values [outer, inner, K] of the rows' type, indices [outer, inner, K]; 1 <= K <= min(V, GSCAN_MAX_TOP).
+ * lse (may be NULL) [outer, inner] = log sum exp of the row (-inf without a word above -inf).
+ * workspace: gscan_top_logits_workspace_bytes(rows, K) bytes (0 for many rows or small vocabularies; 8-byte aligned); it holds
+ * nothing between calls, and calls that may run at the same time need one each. */
+size_t gscan_top_logits_workspace_bytes(const gscan_rows *rows, int K);
+int gscan_top_logits(const gscan_rows *rows, int K, void *values, int32_t *indices, float *lse, void *workspace,
+                     size_t workspace_bytes, void *stream);
+
+/* A teacher's top logits, the labels beside them and the weights of the two terms. */
+typedef struct gscan_distillation {
+    const void *indices;       /* [outer, inner, K] int32 or int64: an index outside [0, V) is no entry (a shorter row);
+                                * an index that comes twice counts with both entries                                      */
+    const void *teacher;       /* [outer, inner, K] the teacher's logits of these words; -inf: probability 0             */
+    const int64_t *labels;     /* [outer, inner], or NULL: every row is live (and hard_weight is 0)                      */
+    int64_t ignore_index;      /* rows with this label, or with one outside [0, V), are not live: they contribute nothing,
+                                * their gradient is 0, and neither their words nor their teacher's are read              */
+    int32_t index_bits;        /* 32 or 64                                                                               */
+    int32_t teacher_type;      /* GSCAN_F32, ...                                                                         */
+    int32_t K;                 /* 1..GSCAN_MAX_TOP                                                                       */
+    int32_t shift_labels;      /* labels are whole sequences: row (o, i) is scored against labels[o, i + 1], the last one
+                                * against 0 (Model.get_loss: seq2seq/model.py:108-115)                                   */
+    float temperature;         /* 1e-3 .. 1e3                                                                            */
+    float soft_weight, hard_weight;
+    int32_t sum_reduction;     /* 0: mean over the live rows (0 when there is none), 1: sum                              */
+} gscan_distillation;
+
+/* With p = softmax(teacher / temperature) over a row's entries, q = softmax(z / temperature), s = softmax(z):
+ *   loss = mean over the live rows of  hard_weight (-log s[label]) + soft_weight temperature^2 sum_k p_k log(p_k / q[index_k])
+ * (a row without entries has no soft term).  stats[4] = [sum -log s[label], live rows, temperature^2-free sum of the
+ * divergences, loss] (a term whose weight is 0 is not computed: its sum is 0).  grad (may be NULL: the loss alone)
+ * [outer, inner, V] of the rows' type, contiguous, receives upstream[0] (device scalar, NULL = 1) times d(loss)/d(logits),
+ * rounded once; it may not overlap the logits.  Two calls give the same bits. */
+size_t gscan_distillation_workspace_bytes(const gscan_rows *rows);
+int gscan_distillation_loss(const gscan_rows *rows, const gscan_distillation *terms, const float *upstream, void *grad,
+                            float *stats, void *workspace, size_t workspace_bytes, void *stream);
+
+/* One step of beam search over `outer` batch rows of `inner` beams (at most GSCAN_MAX_BEAMS): the `inner` best candidates by
+ * scores[b, w] + log_softmax(logits[b, w])[v], ties to the lowest w * V + v, in order.  A beam with finished[b, w] != 0 has
+ * one candidate, itself with its score unchanged and the word `pad`; its logits are not read.  A beam with the score -inf
+ * (a search's first step: every beam but one) is not read either and fills places that nothing else takes, as do candidates
+ * of score -inf (word barred by -inf, NaN), in order of w * V + v.  Logits of +inf have no log_softmax: such a beam's
+ * candidates count as -inf.  Outputs [outer, inner]: score, parent beam, word, finished (the parent was, or word == eos). */
+size_t gscan_beam_select_workspace_bytes(const gscan_rows *rows);
+int gscan_beam_select(const gscan_rows *rows, const float *scores, const uint8_t *finished, int eos, int pad, float *scores_out,
+                      int32_t *parents, int64_t *tokens, uint8_t *finished_out, void *workspace, size_t workspace_bytes,
+                      void *stream);
+
+/* A tensor with one slice per beam: slice (o, b, w, m) of `bytes` adjacent bytes at o * outer stride + (b W + w) * row stride
+ * + m * mid stride (strides in bytes, not negative). */
+typedef struct gscan_state {
+    const void *in;
+    void *out;
+    int64_t outer, mid, bytes;
+    int64_t in_outer, out_outer, in_row, out_row, in_mid, out_mid;
+} gscan_state;
+
+/* out[o, b, w, m] = in[o, b, parents[b, w], m] for every state (any number, 16 to a launch).  A parent outside [0, W) gives
+ * zeros.  out may not overlap in. */
+int gscan_beam_reorder(int B, int W, const int32_t *parents, const gscan_state *states, int count, void *stream);
 
 /* Per-kernel-family timing for roofline reports: when enabled, every launch of a family
  * ("decoder_forward", "decoder_backward", "encoder_forward", "encoder_backward", "gemm", "conv_forward",

@@ -11,7 +11,7 @@ from typing import Optional
 HERE = os.path.dirname(os.path.abspath(__file__))
 # GSCAN_HIP_LIB: development override, used by tools/variants.py to time experimental builds side by side
 LIB_PATH = os.environ.get("GSCAN_HIP_LIB") or os.path.join(HERE, "libgscan_hip.so")
-ABI_VERSION = 14
+ABI_VERSION = 15
 MAX_ENC_LAYERS = 4
 COMM_ID_BYTES = 128
 
@@ -70,6 +70,28 @@ class Masks(C.Structure):
                 ("seed", C.c_uint64), ("stream_id", C.c_uint64)]
 
 
+F32, BF16, F16 = 0, 1, 2          # GSCAN_F32, ...
+MAX_TOP, MAX_BEAMS = 256, 64
+
+
+class Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("type", C.c_int32), ("V", C.c_int32), ("outer", C.c_int64), ("inner", C.c_int64),
+                ("stride_outer", C.c_int64), ("stride_inner", C.c_int64)]
+
+
+class Distillation(C.Structure):
+    _fields_ = [("indices", C.c_void_p), ("teacher", C.c_void_p), ("labels", C.c_void_p), ("ignore_index", C.c_int64),
+                ("index_bits", C.c_int32), ("teacher_type", C.c_int32), ("K", C.c_int32), ("shift_labels", C.c_int32),
+                ("temperature", C.c_float), ("soft_weight", C.c_float), ("hard_weight", C.c_float),
+                ("sum_reduction", C.c_int32)]
+
+
+class State(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("outer", C.c_int64), ("mid", C.c_int64), ("bytes", C.c_int64),
+                ("in_outer", C.c_int64), ("out_outer", C.c_int64), ("in_row", C.c_int64), ("out_row", C.c_int64),
+                ("in_mid", C.c_int64), ("out_mid", C.c_int64)]
+
+
 _vp, _i, _f, _sz, _i64, _u64 = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_int64, C.c_uint64
 
 # name -> (restype, argtypes); every symbol include/gscan_hip.h declares
@@ -116,6 +138,13 @@ PROTOTYPES = {
     "gscan_comm_count": (_i, [_vp, C.POINTER(_i)]),
     "gscan_early_gradients_wait": (_i, [_vp]),
     "gscan_comm_set_early_allreduce": (_i, [_vp, _vp, _sz]),
+    "gscan_top_logits_workspace_bytes": (_sz, [C.POINTER(Rows), _i]),
+    "gscan_top_logits": (_i, [C.POINTER(Rows), _i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "gscan_distillation_workspace_bytes": (_sz, [C.POINTER(Rows)]),
+    "gscan_distillation_loss": (_i, [C.POINTER(Rows), C.POINTER(Distillation), _vp, _vp, _vp, _vp, _sz, _vp]),
+    "gscan_beam_select_workspace_bytes": (_sz, [C.POINTER(Rows)]),
+    "gscan_beam_select": (_i, [C.POINTER(Rows), _vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "gscan_beam_reorder": (_i, [_i, _i, _vp, C.POINTER(State), _i, _vp]),
     "gscan_probe_enable": (_i, [_i]),
     "gscan_probe_reset": (_i, []),
     "gscan_probe_read": (_i, [C.c_char_p, C.POINTER(C.c_double), C.POINTER(C.c_double), C.POINTER(C.c_double),

@@ -18,7 +18,7 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 OBJ = os.path.join(CSRC, "build")
 LIB = os.path.join(HERE, "libgscan_hip.so")
 SOURCES = ["gemm.hip", "gemm_mt.hip", "gemm_ws.hip", "conv.hip", "elementwise.hip", "loss.hip", "lstm_encoder.hip", "decoder.hip", "decoder_any.hip", "attention_grad.hip", "step.hip",
-           "probe.hip", "comm.hip", "capi.hip"]
+           "top_logits.hip", "distill.hip", "beam.hip", "probe.hip", "comm.hip", "capi.hip"]
 # decoder.hip is compiled as four translation units, a quarter of the hidden sizes each (-DGSCAN_DEC_PART=k, csrc/step.h):
 # on one core the file took 80 s of the build's 95
 PARTS = {"decoder.hip": 4}
@@ -38,7 +38,10 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-u
          f"-I{INCLUDE}", f"-I{CSRC}"]
 # per-source extras: the grouped GEMM's problem lookup reads its header from preloaded kernel-argument SGPRs
 EXTRA_FLAGS = {"gemm.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=12"],
-               "gemm_mt.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=12"]}
+               "gemm_mt.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=12"],
+               # no packed fp32 instructions in the operators over rows of logits
+               **{src: ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+                  for src in ("top_logits.hip", "distill.hip", "beam.hip")}}
 
 
 def _hipcc() -> str:

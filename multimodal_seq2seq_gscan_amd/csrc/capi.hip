@@ -1,6 +1,7 @@
 // extern "C" surface of libgscan_hip.so (declared in include/gscan_hip.h).
 #include <string.h>
 
+#include "logits.h"
 #include "step.h"
 
 namespace gscan {
@@ -259,6 +260,38 @@ int gscan_comm_destroy(void *comm) { return comm_destroy(comm); }
 int gscan_comm_count(void *comm, int *nranks) { return comm_count(comm, nranks); }
 int gscan_early_gradients_wait(void *stream) { return early_gradients_wait((hipStream_t)stream); }
 int gscan_comm_set_early_allreduce(void *comm, float *buf, size_t n) { return set_early_allreduce(comm, buf, n); }
+
+size_t gscan_top_logits_workspace_bytes(const gscan_rows *rows, int K) {
+    if (check_rows("top_logits_workspace_bytes", rows) || K < 1) return 0;
+    return top_logits_workspace(*rows, K);
+}
+int gscan_top_logits(const gscan_rows *rows, int K, void *values, int32_t *indices, float *lse, void *workspace,
+                     size_t workspace_bytes, void *stream) {
+    if (int rc = check_rows("top_logits", rows)) return rc;
+    return top_logits(*rows, K, values, indices, lse, workspace, workspace_bytes, (hipStream_t)stream);
+}
+size_t gscan_distillation_workspace_bytes(const gscan_rows *rows) {
+    return check_rows("distillation_workspace_bytes", rows) ? 0 : distillation_workspace(*rows);
+}
+int gscan_distillation_loss(const gscan_rows *rows, const gscan_distillation *terms, const float *upstream, void *grad,
+                            float *stats, void *workspace, size_t workspace_bytes, void *stream) {
+    ARG(terms, "distillation_loss: terms is NULL");
+    if (int rc = check_rows("distillation_loss", rows)) return rc;
+    return distillation_loss(*rows, *terms, upstream, grad, stats, workspace, workspace_bytes, (hipStream_t)stream);
+}
+size_t gscan_beam_select_workspace_bytes(const gscan_rows *rows) {
+    return check_rows("beam_select_workspace_bytes", rows) ? 0 : beam_select_workspace(*rows);
+}
+int gscan_beam_select(const gscan_rows *rows, const float *scores, const uint8_t *finished, int eos, int pad, float *scores_out,
+                      int32_t *parents, int64_t *tokens, uint8_t *finished_out, void *workspace, size_t workspace_bytes,
+                      void *stream) {
+    if (int rc = check_rows("beam_select", rows)) return rc;
+    return beam_select(*rows, scores, finished, eos, pad, scores_out, parents, tokens, finished_out, workspace,
+                       workspace_bytes, (hipStream_t)stream);
+}
+int gscan_beam_reorder(int B, int W, const int32_t *parents, const gscan_state *states, int count, void *stream) {
+    return beam_reorder(B, W, parents, states, count, (hipStream_t)stream);
+}
 
 int gscan_probe_enable(int on) { return probe_enable(on); }
 int gscan_probe_reset(void) { return probe_reset(); }
