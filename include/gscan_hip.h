@@ -367,13 +367,14 @@ typedef struct gscan_distillation {
 
 /* With p = softmax(teacher / temperature) over a row's entries, q = softmax(z / temperature), s = softmax(z):
  *   loss = mean over the live rows of  hard_weight (-log s[label]) + soft_weight temperature^2 sum_k p_k log(p_k / q[index_k])
- * (a row without entries has no soft term).  stats[4] = [sum -log s[label], live rows, temperature^2-free sum of the
- * divergences, loss] (a term whose weight is 0 is not computed: its sum is 0).  grad (may be NULL: the loss alone)
- * [outer, inner, V] of the rows' type, contiguous, receives upstream[0] (device scalar, NULL = 1) times d(loss)/d(logits),
- * rounded once; it may not overlap the logits.  Two calls give the same bits. */
+ * (a row without entries has no soft term), written to loss[0] (NULL, without stats: the gradient alone).  grad (may be NULL: the loss alone) [outer, inner, V] of the
+ * rows' type, contiguous, receives upstream[0] (device scalar, NULL = 1) times d(loss)/d(logits), rounded once; it may not
+ * overlap the logits.  stats (may be NULL) [4] = [sum of the rows' losses, live rows, sum of -log s[label], sum of the
+ * divergences] (of a term whose weight is 0: 0) — what a data-parallel step adds up over its ranks.  Two calls give the same
+ * bits. */
 size_t gscan_distillation_workspace_bytes(const gscan_rows *rows);
 int gscan_distillation_loss(const gscan_rows *rows, const gscan_distillation *terms, const float *upstream, void *grad,
-                            float *stats, void *workspace, size_t workspace_bytes, void *stream);
+                            float *loss, float *stats, void *workspace, size_t workspace_bytes, void *stream);
 
 /* One step of beam search over `outer` batch rows of `inner` beams (at most GSCAN_MAX_BEAMS): the `inner` best candidates by
  * scores[b, w] + log_softmax(logits[b, w])[v], ties to the lowest w * V + v, in order.  A beam with finished[b, w] != 0 has

@@ -141,7 +141,7 @@ PROTOTYPES = {
     "gscan_top_logits_workspace_bytes": (_sz, [C.POINTER(Rows), _i]),
     "gscan_top_logits": (_i, [C.POINTER(Rows), _i, _vp, _vp, _vp, _vp, _sz, _vp]),
     "gscan_distillation_workspace_bytes": (_sz, [C.POINTER(Rows)]),
-    "gscan_distillation_loss": (_i, [C.POINTER(Rows), C.POINTER(Distillation), _vp, _vp, _vp, _vp, _sz, _vp]),
+    "gscan_distillation_loss": (_i, [C.POINTER(Rows), C.POINTER(Distillation), _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "gscan_beam_select_workspace_bytes": (_sz, [C.POINTER(Rows)]),
     "gscan_beam_select": (_i, [C.POINTER(Rows), _vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "gscan_beam_reorder": (_i, [_i, _i, _vp, C.POINTER(State), _i, _vp]),

@@ -42,31 +42,33 @@ __device__ __forceinline__ uint64_t score_key(double score, double z, double lse
 __global__ __launch_bounds__(256) void beam_join_kernel(BeamArgs a) {
     extern __shared__ uint64_t s_key[];          // [entries], then uint32 flat[entries], then int head[lists]
     __shared__ double s_lse[kMaxBeams];
+    __shared__ float s_score[kMaxBeams];
+    __shared__ uint8_t s_done[kMaxBeams];
     const int b = blockIdx.x, tid = threadIdx.x, lists = a.W * a.splits, n = lists * a.K;
     uint32_t *s_flat = (uint32_t *)(s_key + n);
     int *s_head = (int *)(s_flat + n);
     const int64_t row0 = (int64_t)b * a.W;
-    if (tid < a.W && !a.finished[row0 + tid] && a.scores[row0 + tid] != -INFINITY) {
-        const LsePart *part = a.parts + (row0 + tid) * a.splits;
-        float ref = part[0].ref;
-        for (int i = 1; i < a.splits; ++i) ref = fmaxf(ref, part[i].ref);
-        double s = 0.0;
-        for (int i = 0; i < a.splits; ++i) s += part[i].sum * exp((double)part[i].ref - (double)ref);
-        s_lse[tid] = (double)ref + log(s);
+    const uint64_t *keys = a.keys + row0 * a.splits * a.K;
+    // what a beam that is finished or has no score has left there is not looked at
+    const uint64_t early = tid < n ? keys[tid] : 0ull;
+    if (tid < a.W) { s_score[tid] = a.scores[row0 + tid]; s_done[tid] = a.finished[row0 + tid]; }
+    for (int w = tid >> 6; w < a.W; w += 4) {
+        const double lse = join_lse(a.parts + (row0 + w) * a.splits, a.splits);
+        if ((tid & 63) == 0) s_lse[w] = lse;
     }
     for (int l = tid; l < lists; l += 256) s_head[l] = 0;
     __syncthreads();
     for (int i = tid; i < n; i += 256) {
         const int l = i / a.K, k = i - l * a.K, w = l / a.splits, c = l - w * a.splits;
-        const float score = a.scores[row0 + w];
+        const float score = s_score[w];
         uint64_t key = 0;
         uint32_t v = 0;
-        if (a.finished[row0 + w]) {
+        if (s_done[w]) {
             if (c == 0 && k == 0) { key = score_key((double)score, 0.0, 0.0); v = (uint32_t)a.pad; }
         } else if (score == -INFINITY) {
             if (c == 0) { key = order_key64(-INFINITY); v = (uint32_t)k; }
         } else {
-            const uint64_t x = a.keys[row0 * a.splits * a.K + i];
+            const uint64_t x = i == tid ? early : keys[i];
             if (x) { key = score_key((double)score, (double)key_value((uint32_t)(x >> 32)), s_lse[w]); v = ~(uint32_t)x; }
         }
         s_key[i] = key;
@@ -88,19 +90,22 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamArgs a) {
             if (k > best || (k == best && k && f < flat)) { best = k; flat = f; from = l; }
         }
     };
+    auto largest = [](uint32_t x, uint32_t y) { return max(x, y); };
+    auto smallest = [](uint32_t x, uint32_t y) { return min(x, y); };
     refresh();
     for (int place = 0; place < a.W; ++place) {
-        uint64_t k = best;
-        uint32_t f = flat;
-#pragma unroll
-        for (int d = 32; d; d >>= 1) {
-            const uint64_t ok = __shfl_xor(k, d);
-            const uint32_t of = __shfl_xor(f, d);
-            if (ok > k || (ok == k && of < f)) { k = ok; f = of; }
+        // the high words settle it unless two scores come within 2^-20 of each other
+        uint32_t high = wave_reduce((uint32_t)(best >> 32), largest);
+        bool in = (uint32_t)(best >> 32) == high;
+        if (__popcll(__ballot(in)) > 1) {
+            const uint32_t low = wave_reduce(in ? (uint32_t)best : 0u, largest);
+            in = in && (uint32_t)best == low;
+            const uint32_t first = wave_reduce(in ? flat : ~0u, smallest);
+            in = in && flat == first;
         }
-        if (from >= 0 && best == k && flat == f) {       // one lane: candidates differ in `flat`
+        if (in && from >= 0) {                       // one lane: candidates differ in `flat`
             s_head[from] += 1;
-            put_beam(a, b, place, k, f);
+            put_beam(a, b, place, best, flat);
             refresh();
         }
     }

@@ -274,10 +274,10 @@ size_t gscan_distillation_workspace_bytes(const gscan_rows *rows) {
     return check_rows("distillation_workspace_bytes", rows) ? 0 : distillation_workspace(*rows);
 }
 int gscan_distillation_loss(const gscan_rows *rows, const gscan_distillation *terms, const float *upstream, void *grad,
-                            float *stats, void *workspace, size_t workspace_bytes, void *stream) {
+                            float *loss, float *stats, void *workspace, size_t workspace_bytes, void *stream) {
     ARG(terms, "distillation_loss: terms is NULL");
     if (int rc = check_rows("distillation_loss", rows)) return rc;
-    return distillation_loss(*rows, *terms, upstream, grad, stats, workspace, workspace_bytes, (hipStream_t)stream);
+    return distillation_loss(*rows, *terms, upstream, grad, loss, stats, workspace, workspace_bytes, (hipStream_t)stream);
 }
 size_t gscan_beam_select_workspace_bytes(const gscan_rows *rows) {
     return check_rows("beam_select_workspace_bytes", rows) ? 0 : beam_select_workspace(*rows);

@@ -11,12 +11,21 @@
 // one more reduction beside the row's sums does it.  Sums are in 32 bits within a row and in 64 across rows.
 // The few words that the teacher or the label names are stored a second time behind the row, with their share taken off:
 // same workgroup, behind a barrier; an index that comes twice is handled once, by its first entry, with both shares.
+#include <type_traits>
+
 #include "logits.h"
 
 namespace gscan {
 
 namespace {
 constexpr int kCountBlocks = 64;
+// Up to so many rows, the launch that needs the number of live rows counts the labels itself, in every workgroup (a launch
+// less: 22.8 for 27.1 us at 5120 rows of 9 words); longer rows fill the chip with workgroups, and theirs come from a launch
+// before them (4088 rows of 32000 words: 134 for 152 us).
+constexpr int kCountThere = 8192, kCountThereLong = 256;
+// Gradients from so many bytes on are stored past the caches (non-temporal), as they leave the 256 MB of the last one before
+// anything reads them: 262 MB 125 -> 115 us; 131 MB would go from 73 to 76.
+constexpr int64_t kFarGradient = 192 << 20;
 
 struct DistillArgs {
     Rows rows;
@@ -27,11 +36,16 @@ struct DistillArgs {
     const int64_t *labels; int64_t ignore; int shift;
     float inv_tau, soft, hard;
     float soft_grad;                   // soft weight times tau
-    const int *live;                   // kCountBlocks partial counts (mean), or NULL (sum)
+    int power;                         // tau where it is 2, 3 or 4
+    int sum;                           // the gradient of the sum, not of the mean
+    const int *live;                   // kCountBlocks partial counts of the live rows, or NULL: counted where they are needed
     const float *upstream;             // or NULL: 1
     char *grad;                        // [rows][V], or NULL
+    int far;                           // stored past the caches
     double *part;                      // [workgroups][3]: hard loss, soft loss, live rows
 };
+
+__device__ __forceinline__ bool is_live(const DistillArgs &a, int64_t y) { return y != a.ignore && (uint64_t)y < (uint64_t)a.rows.V; }
 
 // the label of row r, or -1 when the row is not live; -2 when there are no labels and every row is
 __device__ __forceinline__ int row_label(const DistillArgs &a, int r) {
@@ -39,7 +53,7 @@ __device__ __forceinline__ int row_label(const DistillArgs &a, int r) {
     int64_t y;
     if (a.shift) y = (r + 1) % a.rows.inner ? a.labels[r + 1] : (int64_t)0;       // the sequence moved left by one, 0 behind it
     else y = a.labels[r];
-    return y != a.ignore && y >= 0 && y < a.rows.V ? (int)y : -1;
+    return is_live(a, y) ? (int)y : -1;
 }
 
 __device__ __forceinline__ float teacher_value(const DistillArgs &a, int64_t at) {
@@ -53,29 +67,40 @@ __device__ __forceinline__ int teacher_index(const DistillArgs &a, int64_t at) {
     return i >= 0 && i < a.rows.V ? (int)i : -1;
 }
 
-// 1 / live rows (or 1) times the upstream gradient; every lane of the wave takes part
-__device__ __forceinline__ float gradient_scale(const DistillArgs &a) {
-    float s = a.upstream ? a.upstream[0] : 1.f;
-    if (a.live) {
-        const int n = wave_reduce(a.live[threadIdx.x & 63], [](int x, int y) { return x + y; });
-        s = n > 0 ? s / (float)n : 0.f;
+// Live rows among those that this thread looks at, of `threads` threads.  Of shifted labels, the first of every sequence is
+// nobody's and a 0 stands behind the last.
+__device__ __forceinline__ int count_live(const DistillArgs &a, int first, int threads) {
+    int n = 0;
+    if (!a.labels) {
+        for (int r = first; r < a.count; r += threads) ++n;
+        return n;
     }
-    return s;
+    for (int r = first; r < a.count; r += threads) n += is_live(a, a.labels[r]) ? 1 : 0;
+    if (a.shift) {
+        const int behind = is_live(a, 0) ? 1 : 0;
+        for (int o = first; o < a.count / a.rows.inner; o += threads) n += behind - (is_live(a, a.labels[(int64_t)o * a.rows.inner]) ? 1 : 0);
+    }
+    return n;
+}
+
+// 1 / live rows (or 1) times the upstream gradient: from the count that a launch before this one has left, or (few rows) from
+// the labels themselves.
+__device__ __forceinline__ float over_live(const DistillArgs &a, int n) {
+    const float s = a.upstream ? a.upstream[0] : 1.f;
+    return a.sum ? s : n > 0 ? s / (float)n : 0.f;
 }
 
 // live rows, in kCountBlocks parts
 __global__ __launch_bounds__(256) void distill_count_kernel(DistillArgs a, int *live) {
     __shared__ int s[4];
-    int n = 0;
-    for (int r = blockIdx.x * 256 + threadIdx.x; r < a.count; r += kCountBlocks * 256) n += row_label(a, r) != -1 ? 1 : 0;
+    int n = count_live(a, blockIdx.x * 256 + threadIdx.x, kCountBlocks * 256);
     n = wave_reduce(n, [](int x, int y) { return x + y; });
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = n;
     __syncthreads();
     if (threadIdx.x == 0) live[blockIdx.x] = s[0] + s[1] + s[2] + s[3];
 }
 
-// stats: hard loss sum, live rows, soft loss sum (with tau^2), loss
-__global__ __launch_bounds__(1024) void distill_finish_kernel(const double *part, int n, float soft, float hard, int mean, float *stats) {
+__global__ __launch_bounds__(1024) void distill_finish_kernel(const double *part, int n, float soft, float hard, int mean, float *loss, float *stats) {
     __shared__ double s[3][16];
     double v[3] = {0.0, 0.0, 0.0};
     for (int i = threadIdx.x; i < n; i += 1024) {
@@ -92,85 +117,169 @@ __global__ __launch_bounds__(1024) void distill_finish_kernel(const double *part
             v[k] = s[k][0];
             for (int w = 1; w < 16; ++w) v[k] += s[k][w];
         }
-        const double loss = (hard != 0.f ? (double)hard * v[0] : 0.0) + (soft != 0.f ? (double)soft * v[1] : 0.0);
-        stats[0] = (float)v[0]; stats[1] = (float)v[2]; stats[2] = (float)v[1];
-        stats[3] = (float)(mean ? loss / (v[2] > 0.0 ? v[2] : 1.0) : loss);
+        const double sum = (hard != 0.f ? (double)hard * v[0] : 0.0) + (soft != 0.f ? (double)soft * v[1] : 0.0);
+        loss[0] = (float)(mean ? sum / (v[2] > 0.0 ? v[2] : 1.0) : sum);
+        if (stats) { stats[0] = (float)sum; stats[1] = (float)v[2]; stats[2] = (float)v[0]; stats[3] = (float)v[1]; }
     }
 }
 
 template <int TPB>
 struct RowShared {
-    int index[kMaxTop + 1];
-    float share[kMaxTop + 1];        // e_k
-    float red[5][TPB / 64 + 1];
+    alignas(16) int index[kMaxTop];
+    float share[kMaxTop];                        // e_k
+    // words whose value is stored a second time, the label's last; and which of them lie in a wave's pieces
+    int word[kMaxTop + 1];
+    float value[kMaxTop + 1];
+    uint16_t list[TPB / 64][kMaxTop + 1];
+    int listed[TPB / 64];
+    float top[2][TPB / 64], sums[4][TPB / 64], live[TPB / 64];
 };
 
-template <int TPB, int N, class Op>
-__device__ __forceinline__ void block_reduce(RowShared<TPB> &sh, float (&v)[N], Op op) {
-    const int wave = threadIdx.x >> 6;
+// Sums (or maxima) of N values over the workgroup: through a place of its own in LDS, so one barrier does.
+template <int TPB, bool MAX, int N>
+__device__ __forceinline__ void block_reduce(float (&place)[N][TPB / 64], float (&v)[N]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = wave_reduce(v[i], op);
+    for (int i = 0; i < N; ++i) v[i] = MAX ? wave_max(v[i]) : wave_sum(v[i]);
     if constexpr (TPB > 64) {
         if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) sh.red[i][wave] = v[i];
+            for (int i = 0; i < N; ++i) place[i][threadIdx.x >> 6] = v[i];
         }
-        __syncthreads();
+    }
+    lds_barrier();
+    if constexpr (TPB > 64) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            v[i] = sh.red[i][0];
-            for (int w = 1; w < TPB / 64; ++w) v[i] = op(v[i], sh.red[i][w]);
+            v[i] = place[i][0];
+#pragma unroll
+            for (int w = 1; w < TPB / 64; ++w) v[i] = MAX ? fmaxf(v[i], place[i][w]) : v[i] + place[i][w];
         }
-        __syncthreads();
     }
 }
 
-// One workgroup per row.  NR > 0: the row in NR 16-byte pieces per thread; NR = 0: the row is read again for every use (rows
-// longer than the registers of a workgroup of 1024).
-// TWO: two different exponentials a word (both terms, tau != 1); otherwise one serves the term or both.
-template <class T, int TPB, int NR, bool TWO, bool GRAD>
-__global__ __launch_bounds__(TPB) void distill_row_kernel(DistillArgs a) {
+template <int TPB>
+__device__ __forceinline__ float gradient_scale(const DistillArgs &a, RowShared<TPB> &sh) {
+    if (a.sum) return over_live(a, 0);
+    if (a.live) return over_live(a, (int)wave_sum((float)a.live[threadIdx.x & 63]));
+    const float n = wave_sum((float)count_live(a, threadIdx.x, TPB));       // at most 2^24 rows: exact
+    if ((threadIdx.x & 63) == 0) sh.live[threadIdx.x >> 6] = n;
+    lds_barrier();
+    float all = 0.f;
+    for (int w = 0; w < TPB / 64; ++w) all += sh.live[w];
+    return over_live(a, (int)all);
+}
+
+// How a word's two exponentials, exp((z - z_max) / tau) for the soft term and exp(z - z_max) for the hard one, are had.
+// kOne: one of them is all there is (a single term, or tau = 1).  kPower: tau is 2, 3 or 4, the second is the first one's
+// power.  kTwo: two.
+enum Exponentials { kOne, kPower, kTwo };
+
+// In powers of two and relative to the row's maximum.  NEAR: as 2^(a z + b), b = -a z_max rounded: one multiply-add a word;
+// every exponential of a row is off by the same 2^delta, which the quotients do not show and the logarithms take off again.
+// Otherwise (a maximum so far out that delta grows, a row of the type's lowest value say) the distance comes first.
+template <int E, bool NEAR>
+struct Exponents {
+    float zmax, a0, a1, b0, b1;
+    int power;
+    // first: the first exponential.  other: the second one; kPower: what the first is multiplied by to give it.
+    template <int N>
+    __device__ __forceinline__ void operator()(const float (&z)[N], float (&first)[N], float (&other)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            first[i] = __builtin_amdgcn_exp2f(NEAR ? fmaf(z[i], a0, b0) : (z[i] - zmax) * a0);
+            if constexpr (E == kTwo) other[i] = __builtin_amdgcn_exp2f(NEAR ? fmaf(z[i], a1, b1) : (z[i] - zmax) * a1);
+            if constexpr (E == kPower) other[i] = first[i];
+        }
+        if constexpr (E == kPower) {
+            if (power > 2) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) other[i] *= first[i];
+            }
+            if (power > 3) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) other[i] *= first[i];
+            }
+        }
+    }
+    template <int N>
+    __device__ __forceinline__ void add(const float (&z)[N], float &s0, float &s1) const {
+        float first[N], other[N];
+        (*this)(z, first, other);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            s0 += first[i];
+            if constexpr (E == kTwo) s1 += other[i];
+            if constexpr (E == kPower) s1 = fmaf(first[i], other[i], s1);
+        }
+    }
+    // c0 first exponential + c1 second one
+    template <int N>
+    __device__ __forceinline__ void mix(const float (&z)[N], float c0, float c1, float (&g)[N]) const {
+        float first[N], other[N];
+        (*this)(z, first, other);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (E == kOne) g[i] = c0 * first[i];
+            if constexpr (E == kTwo) g[i] = fmaf(c1, other[i], c0 * first[i]);
+            if constexpr (E == kPower) g[i] = first[i] * fmaf(c1, other[i], c0);
+        }
+    }
+};
+
+// Rows of 16-byte pieces of 64 words and more, a workgroup per row.
+//
+// NR > 0: the row stays in NR pieces per thread.
+// NR = 0: the row is read a second time for the gradient, and its maximum and sums come from one pass in which a thread
+// rescales its sums when its maximum grows (rows longer than the registers hold, and the loss alone).
+//
+// The words that the teacher or the label names get their value a second time, from the wave that has stored their piece:
+// a wave's stores to one place stay in order, so nothing waits for the row.
+template <class T, int TPB, int NR, int E, bool GRAD>
+__global__ __launch_bounds__(TPB) __attribute__((amdgpu_waves_per_eu(4))) void distill_row_kernel(DistillArgs a) {
     __shared__ RowShared<TPB> sh;
     constexpr int NK = TPB >= kMaxTop ? 1 : kMaxTop / TPB;      // teacher entries per thread
-    const int tid = threadIdx.x, r = blockIdx.x, V = a.rows.V;
-    const char *row = a.rows.row(r);
-    const int pieces = V / T::vec, rest = V - pieces * T::vec;       // whole 16-byte pieces, and words behind them: one a thread
-    const int label = row_label(a, r);
+    constexpr int N = T::vec;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, V = a.rows.V;
+    const int pieces = V / N, rest = V - pieces * N;            // whole 16-byte pieces, and words behind them: one a thread
+    const int r = blockIdx.x, label = row_label(a, r);
+    double *part = a.part + 3 * (int64_t)r;
     char *out = GRAD ? a.grad + (int64_t)r * V * T::bytes : nullptr;
+    auto store = [&](char *to, const Raw &w) {
+        if (NR == 0 || a.far) store16<T, true>(to, w);
+        else store16<T>(to, w);
+    };
     if (label == -1) {                 // not live: neither its words nor its teacher's are read
         if constexpr (GRAD) {
-            for (int p = tid; p < pieces; p += TPB) store16<T>(out + (int64_t)p * 16, Raw{{0, 0, 0, 0}});
-            if (tid < rest) store1<T>(out, pieces * T::vec + tid, 0.f);
+            for (int p = tid; p < pieces; p += TPB) store(out + (int64_t)p * 16, Raw{{0, 0, 0, 0}});
+            if (tid < rest) store1<T>(out, pieces * N + tid, 0.f);
         }
-        if (tid == 0) { a.part[3 * (int64_t)r] = 0.0; a.part[3 * (int64_t)r + 1] = 0.0; a.part[3 * (int64_t)r + 2] = 0.0; }
+        if (tid < 3) part[tid] = 0.0;
         return;
     }
+    const char *row = a.rows.row(r);
+    // piece i of this thread begins at byte 16 (tid + i TPB): a uniform address per i and one offset for all of them
+    const uint32_t at16 = (uint32_t)tid * 16;
+    auto has = [&](int i) { return tid < pieces - i * TPB; };
     Raw x[NR ? NR : 1];
 #pragma unroll
     for (int i = 0; i < NR; ++i)
-        if (i * TPB < pieces) x[i] = load16<T>(row + (int64_t)min(tid + i * TPB, pieces - 1) * 16);
-    const float last = tid < rest ? load1<T>(row, pieces * T::vec + tid) : -INFINITY;
-    // f(16 bytes, piece number) for every piece of this thread
-    auto each = [&](auto f) {
-        if constexpr (NR > 0) {
-#pragma unroll
-            for (int i = 0; i < NR; ++i)
-                if (i * TPB < pieces && tid + i * TPB < pieces) f(x[i], tid + i * TPB);
-        } else {
-            for (int p = tid; p < pieces; p += TPB) f(load16<T>(row + (int64_t)p * 16), p);
-        }
-    };
-
-    // The compiler would keep the widened words from one use to the next (twice the registers for 16-bit words, and spills):
-    // behind this the pieces are new values to it.
+        if (has(i)) x[i] = load16<T, true>(row + i * TPB * 16 + at16);
+    const float last[1] = {tid < rest ? load1<T>(row, pieces * N + tid) : -INFINITY};
+    // The compiler would keep the widened words from one use to the next (twice the registers for 16-bit words, and
+    // spills): behind this the pieces are new values to it.
     auto hide = [&]() {
 #pragma unroll
-        for (int i = 0; i < NR; ++i) asm volatile("" : "+v"(x[i].w[0]), "+v"(x[i].w[1]), "+v"(x[i].w[2]), "+v"(x[i].w[3]));
+        for (int i = 0; i < NR; ++i)
+            asm volatile("" : "+v"(x[i].w[0]), "+v"(x[i].w[1]), "+v"(x[i].w[2]), "+v"(x[i].w[3]));
+    };
+    auto widen = [](const Raw &w, float (&z)[N]) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) z[e] = element<T>(w, e);
     };
 
     int idx[NK];
     float t[NK], zk[NK];
-    float top[2] = {-INFINITY, -INFINITY};        // of the row, of the teacher's entries
+    float top[2] = {last[0], -INFINITY};          // of the row, of the teacher's entries
 #pragma unroll
     for (int j = 0; j < NK; ++j) {
         const int k = tid + j * TPB;
@@ -179,34 +288,93 @@ __global__ __launch_bounds__(TPB) void distill_row_kernel(DistillArgs a) {
             const int64_t at = (int64_t)r * a.K + k;
             idx[j] = teacher_index(a, at);
             if (idx[j] >= 0) { t[j] = teacher_value(a, at); zk[j] = load1<T>(row, idx[j]); }
-            sh.index[k] = idx[j];
         }
+        if (GRAD && k < kMaxTop) sh.index[k] = idx[j];
         top[1] = fmaxf(top[1], t[j]);
     }
+    if (GRAD && tid < TPB / 64) sh.listed[tid] = 0;
     const float zy = label >= 0 ? load1<T>(row, label) : 0.f;
-    each([&](const Raw &w, int) {
+
+    const float a0 = (E != kOne || a.soft != 0.f ? a.inv_tau : 1.f) * kLog2e, a1 = kLog2e;
+    float sums[4] = {0.f, 0.f, 0.f, 0.f};         // sum of the first exponential, of the second, A, B
+    if constexpr (NR > 0) {
 #pragma unroll
-        for (int e = 0; e < T::vec; ++e) top[0] = fmaxf(top[0], element<T>(w, e));
-    });
-    top[0] = fmaxf(top[0], last);
-    block_reduce<TPB>(sh, top, [](float p, float q) { return fmaxf(p, q); });
+        for (int i = 0; i < NR; ++i)
+            if (has(i)) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) top[0] = fmaxf(top[0], element<T>(x[i], e));
+            }
+    } else {
+        float ref = fmaxf(last[0], -FLT_MAX);
+        Exponents<E, false> ex{ref, a0, a1, 0.f, 0.f, a.power};
+        auto grow = [&](float m) {
+            if (m > ref) {
+                const float d = ref - m;
+                sums[0] *= __builtin_amdgcn_exp2f(d * a0);
+                if constexpr (E != kOne) sums[1] *= __builtin_amdgcn_exp2f(d * a1);
+                ref = m;
+            }
+            ex.zmax = ref;
+        };
+        auto add = [&](const Raw &w) {
+            float z[N];
+            widen(w, z);
+            ex.add(z, sums[0], sums[1]);
+        };
+        constexpr int U = 4;
+        int p = tid;
+        for (; p + (U - 1) * TPB < pieces; p += U * TPB) {
+            Raw w[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) w[u] = load16<T, !GRAD>(row + (int64_t)(p + u * TPB) * 16);
+            float m = ref;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < N; ++e) m = fmaxf(m, element<T>(w[u], e));
+            grow(m);
+#pragma unroll
+            for (int u = 0; u < U; ++u) add(w[u]);
+        }
+        for (; p < pieces; p += TPB) {
+            const Raw w = load16<T>(row + (int64_t)p * 16);
+            float m = ref;
+#pragma unroll
+            for (int e = 0; e < N; ++e) m = fmaxf(m, element<T>(w, e));
+            grow(m);
+            add(w);
+        }
+        top[0] = ref;
+    }
+    const float mine = top[0];
+    block_reduce<TPB, true>(sh.top, top);
     hide();
     const float zmax = top[0], tmax = top[1];
-
-    // exponents in powers of two, of the distance from the maximum: finite also where every word is the type's lowest
-    const float a0 = (TWO || a.soft != 0.f ? a.inv_tau : 1.f) * kLog2e, a1 = kLog2e;
-    float sums[4] = {0.f, 0.f, 0.f, 0.f};         // sum of the first exponential, of the second, A, B
-    each([&](const Raw &w, int) {
+    const float b0 = -zmax * a0, b1 = -zmax * a1;
+    const bool near = NR > 0 && fabsf(b0) < 1048576.f && fabsf(b1) < 1048576.f;       // delta below 2^-4 then
+    const Exponents<E, true> fast{zmax, a0, a1, b0, b1, a.power};
+    const Exponents<E, false> plain{zmax, a0, a1, b0, b1, a.power};
+    if (near) {
 #pragma unroll
-        for (int e = 0; e < T::vec; ++e) {
-            const float d = element<T>(w, e) - zmax;
-            sums[0] += __builtin_amdgcn_exp2f(d * a0);
-            if constexpr (TWO) sums[1] += __builtin_amdgcn_exp2f(d * a1);
+        for (int i = 0; i < NR; ++i)
+            if (has(i)) {
+                float z[N];
+                widen(x[i], z);
+                fast.add(z, sums[0], sums[1]);
+            }
+        if (tid < rest) fast.add(last, sums[0], sums[1]);
+    } else {
+        if constexpr (NR > 0) {
+            for (int p = tid; p < pieces; p += TPB) {
+                float z[N];
+                widen(load16<T>(row + (int64_t)p * 16), z);
+                plain.add(z, sums[0], sums[1]);
+            }
+        } else {
+            sums[0] *= __builtin_amdgcn_exp2f((mine - zmax) * a0);
+            if constexpr (E != kOne) sums[1] *= __builtin_amdgcn_exp2f((mine - zmax) * a1);
         }
-    });
-    if (tid < rest) {
-        sums[0] += __builtin_amdgcn_exp2f((last - zmax) * a0);
-        if constexpr (TWO) sums[1] += __builtin_amdgcn_exp2f((last - zmax) * a1);
+        if (tid < rest) plain.add(last, sums[0], sums[1]);
     }
     float share[NK];
 #pragma unroll
@@ -218,51 +386,95 @@ __global__ __launch_bounds__(TPB) void distill_row_kernel(DistillArgs a) {
             sums[2] += share[j];
             sums[3] += share[j] * (d - (zk[j] - zmax) * a.inv_tau);
         }
-        if (k < a.K) sh.share[k] = share[j];
+        if (GRAD && k < a.K) sh.share[k] = share[j];
     }
-    block_reduce<TPB>(sh, sums, [](float p, float q) { return p + q; });
-    const float s0 = sums[0], s1 = TWO ? sums[1] : sums[0], A = sums[2], B = sums[3];
+    block_reduce<TPB, false>(sh.sums, sums);
+    const float s0 = sums[0], s1 = E != kOne ? sums[1] : sums[0], A = sums[2], B = sums[3];
     if (tid == 0) {
-        const float hard = a.hard != 0.f ? logf(s1) - (zy - zmax) : 0.f;
-        const float soft = a.soft != 0.f && A != 0.f ? B / A - logf(A) + logf(s0) : 0.f;
-        a.part[3 * (int64_t)r] = (double)hard;
-        a.part[3 * (int64_t)r + 1] = (double)soft;
-        a.part[3 * (int64_t)r + 2] = 1.0;
+        // the row's sums without the common factor 2^delta (its power in the second one)
+        const float off0 = near ? fmaf(zmax, a0, b0) * 0.6931471805599453f : 0.f;
+        const float off1 = E == kPower ? off0 * (float)a.power : E == kTwo && near ? fmaf(zmax, a1, b1) * 0.6931471805599453f : off0;
+        part[0] = a.hard != 0.f ? (double)(logf(s1) - off1 - (zy - zmax)) : 0.0;
+        part[1] = a.soft != 0.f && A != 0.f ? (double)(B / A - logf(A) + (logf(s0) - off0)) : 0.0;
+        part[2] = 1.0;
     }
     if constexpr (GRAD) {
         hide();
-        const float scale = gradient_scale(a);
+        const float scale = gradient_scale<TPB>(a, sh);
         const float soft = a.soft != 0.f && A != 0.f ? a.soft_grad * scale : 0.f, hard = a.hard != 0.f ? a.hard * scale : 0.f;
-        const float c0 = TWO ? soft / s0 : (soft + hard) / s0, c1 = TWO ? hard / s1 : 0.f;
-        auto density = [&](float z) {
-            const float d = z - zmax;
-            float g = c0 * __builtin_amdgcn_exp2f(d * a0);
-            if constexpr (TWO) g = fmaf(c1, __builtin_amdgcn_exp2f(d * a1), g);
-            return g;
+        const float c0 = E != kOne ? soft / s0 : (soft + hard) / s0, c1 = E != kOne ? hard / s1 : 0.f;
+        auto density = [&](float v) {
+            const float z[1] = {v};
+            float g[1];
+            if (near) fast.mix(z, c0, c1, g);
+            else plain.mix(z, c0, c1, g);
+            return g[0];
         };
-        each([&](const Raw &w, int p) {
-            float g[T::vec];
-#pragma unroll
-            for (int e = 0; e < T::vec; ++e) g[e] = density(element<T>(w, e));
-            store16<T>(out + (int64_t)p * 16, pack<T>(g));
-        });
-        if (tid < rest) store1<T>(out, pieces * T::vec + tid, density(last));
-        __syncthreads();                 // the row is stored: the named words follow
+        // the named words' values; an index that comes twice is left to its first entry, with both shares
+        auto name = [&](int k, int v, float value) {
+            const int p = v / N, owner = (p < pieces ? p & (TPB - 1) : v - pieces * N) >> 6;
+            sh.word[k] = v;
+            sh.value[k] = value;
+            sh.list[owner][atomicAdd(&sh.listed[owner], 1)] = (uint16_t)k;
+        };
         const float soft_share = A != 0.f ? soft / A : 0.f;
 #pragma unroll
         for (int j = 0; j < NK; ++j) {
             const int k = tid + j * TPB;
-            if (k >= a.K || idx[j] < 0) continue;
-            float named = 0.f;
+            if (idx[j] < 0) continue;
+            int same = 0;
+            for (int i = 0; i < a.K; i += 4) {
+                const int4 q = *(const int4 *)&sh.index[i];       // behind K: -1
+                same += (q.x == idx[j]) + (q.y == idx[j]) + (q.z == idx[j]) + (q.w == idx[j]);
+            }
+            float named = share[j];
             bool first = true;
-            for (int i = 0; i < a.K; ++i)
-                if (sh.index[i] == idx[j]) { first = first && i >= k; named += sh.share[i]; }
-            if (first) store1<T>(out, idx[j], density(zk[j]) - soft_share * named - (idx[j] == label ? hard : 0.f));
+            if (same > 1) {
+                named = 0.f;
+                for (int i = 0; i < a.K; ++i)
+                    if (sh.index[i] == idx[j]) { first = first && i >= k; named += sh.share[i]; }
+            }
+            if (first) name(k, idx[j], density(zk[j]) - soft_share * named - (idx[j] == label ? hard : 0.f));
         }
-        if (tid == 0 && label >= 0 && hard != 0.f) {
+        if (wave == TPB / 64 - 1 && label >= 0 && hard != 0.f) {
             bool named = false;
-            for (int i = 0; i < a.K; ++i) named = named || sh.index[i] == label;
-            if (!named) store1<T>(out, label, density(zy) - hard);
+            for (int i = lane; i < a.K; i += 64) named = named || sh.index[i] == label;
+            if (!__ballot(named) && lane == 0) name(kMaxTop, label, density(zy) - hard);
+        }
+        if (near) {
+#pragma unroll
+            for (int i = 0; i < NR; ++i)
+                if (has(i)) {
+                    float z[N], g[N];
+                    widen(x[i], z);
+                    fast.mix(z, c0, c1, g);
+                    store(out + i * TPB * 16 + at16, pack<T>(g));
+                }
+        } else {
+            constexpr int U = 4;
+            auto put = [&](const Raw &w, int p) {
+                float z[N], g[N];
+                widen(w, z);
+                plain.mix(z, c0, c1, g);
+                store(out + (int64_t)p * 16, pack<T>(g));
+            };
+            int p = tid;
+            if constexpr (NR == 0) {
+                for (; p + (U - 1) * TPB < pieces; p += U * TPB) {
+                    Raw w[U];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) w[u] = load16<T, true>(row + (int64_t)(p + u * TPB) * 16);
+#pragma unroll
+                    for (int u = 0; u < U; ++u) put(w[u], p + u * TPB);
+                }
+            }
+            for (; p < pieces; p += TPB) put(load16<T>(row + (int64_t)p * 16), p);
+        }
+        if (tid < rest) store1<T>(out, pieces * N + tid, density(last[0]));
+        lds_barrier();
+        for (int i = lane; i < sh.listed[wave]; i += 64) {
+            const int k = sh.list[wave][i];
+            store1<T>(out, sh.word[k], sh.value[k]);
         }
     }
 }
@@ -271,7 +483,8 @@ __global__ __launch_bounds__(TPB) void distill_row_kernel(DistillArgs a) {
 template <class T, int L, bool GRAD>
 __global__ __launch_bounds__(256) void distill_small_kernel(DistillArgs a) {
     extern __shared__ float entries[];
-    __shared__ double s_part[4][3];
+    __shared__ float s_part[4][3];
+    __shared__ int s_live[4];
     constexpr int R = 256 / L;
     const int slot = threadIdx.x / L, v = threadIdx.x & (L - 1), r = blockIdx.x * R + slot, V = a.rows.V, K = a.K;
     float *share = entries + slot * K;
@@ -316,7 +529,15 @@ __global__ __launch_bounds__(256) void distill_small_kernel(DistillArgs a) {
     const float s0 = lanes(e0, plus), s1 = lanes(e1, plus);
     const float zy = label >= 0 ? __shfl(z, label, L) : 0.f;
     if constexpr (GRAD) {
-        const float scale = gradient_scale(a);
+        int n = 0;
+        if (!a.sum) n = a.live ? a.live[threadIdx.x & 63] : count_live(a, threadIdx.x, 256);
+        n = wave_reduce(n, [](int x, int y) { return x + y; });
+        if (!a.sum && !a.live) {
+            if ((threadIdx.x & 63) == 0) s_live[threadIdx.x >> 6] = n;
+            __syncthreads();
+            n = s_live[0] + s_live[1] + s_live[2] + s_live[3];
+        }
+        const float scale = over_live(a, n);
         float g = 0.f;
         if (in) {
             if (hard_on) g = a.hard * scale * (e1 / s1 - (v == label ? 1.f : 0.f));
@@ -328,21 +549,21 @@ __global__ __launch_bounds__(256) void distill_small_kernel(DistillArgs a) {
         }
         if (r < a.count && v < V) store1<T>(a.grad, (int64_t)r * V + v, g);
     }
-    double part[3] = {0.0, 0.0, 0.0};
+    float part[3] = {0.f, 0.f, 0.f};
     if (live && v == 0) {
-        part[0] = hard_on ? (double)(logf(s1) - (zy - zmax)) : 0.0;
-        part[1] = soft_on && A != 0.f ? (double)(B / A - logf(A) + logf(s0)) : 0.0;
-        part[2] = 1.0;
+        part[0] = hard_on ? logf(s1) - (zy - zmax) : 0.f;
+        part[1] = soft_on && A != 0.f ? B / A - logf(A) + logf(s0) : 0.f;
+        part[2] = 1.f;
     }
+    wave_sum_n(part);
+    if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-        part[k] = wave_reduce(part[k], [](double x, double y) { return x + y; });
-        if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6][k] = part[k];
+        for (int k = 0; k < 3; ++k) s_part[threadIdx.x >> 6][k] = part[k];
     }
     __syncthreads();
     if (threadIdx.x < 3)
-        a.part[3 * (int64_t)blockIdx.x + threadIdx.x] =
-            s_part[0][threadIdx.x] + s_part[1][threadIdx.x] + s_part[2][threadIdx.x] + s_part[3][threadIdx.x];
+        a.part[3 * (int64_t)blockIdx.x + threadIdx.x] = (double)s_part[0][threadIdx.x] + (double)s_part[1][threadIdx.x] +
+                                                        (double)s_part[2][threadIdx.x] + (double)s_part[3][threadIdx.x];
 }
 
 int small_lanes(int V) { return V <= 8 ? 8 : V <= 16 ? 16 : V <= 32 ? 32 : 64; }
@@ -361,13 +582,13 @@ int launch_small(const DistillArgs &a, hipStream_t stream) {
     return 0;
 }
 
-template <class T, int TPB, int NR>
-int launch_row(const DistillArgs &a, bool two, hipStream_t stream) {
+template <class T, int TPB, int NR, bool GRAD>
+int launch_row(const DistillArgs &a, hipStream_t stream) {
     const dim3 grid(a.count), block(TPB);
-    if (two && a.grad) hipLaunchKernelGGL((distill_row_kernel<T, TPB, NR, true, true>), grid, block, 0, stream, a);
-    else if (two) hipLaunchKernelGGL((distill_row_kernel<T, TPB, NR, true, false>), grid, block, 0, stream, a);
-    else if (a.grad) hipLaunchKernelGGL((distill_row_kernel<T, TPB, NR, false, true>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((distill_row_kernel<T, TPB, NR, false, false>), grid, block, 0, stream, a);
+    const bool two = a.hard != 0.f && a.soft != 0.f && a.inv_tau != 1.f;
+    if (two && a.power) hipLaunchKernelGGL((distill_row_kernel<T, TPB, NR, kPower, GRAD>), grid, block, 0, stream, a);
+    else if (two) hipLaunchKernelGGL((distill_row_kernel<T, TPB, NR, kTwo, GRAD>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((distill_row_kernel<T, TPB, NR, kOne, GRAD>), grid, block, 0, stream, a);
     GSCAN_LAUNCHED("distill_row_kernel");
     return 0;
 }
@@ -383,13 +604,16 @@ int launch_type(const DistillArgs &a, hipStream_t stream) {
             default: return launch_small<T, 64>(a, stream);
         }
     }
-    const bool two = a.hard != 0.f && a.soft != 0.f && a.inv_tau != 1.f;
     const int pieces = V / T::vec;
-    if (pieces <= 64 * 8) return launch_row<T, 64, 8>(a, two, stream);
-    if (pieces <= 256 * 16) return launch_row<T, 256, 16>(a, two, stream);
-    if (pieces <= 512 * 16) return launch_row<T, 512, 16>(a, two, stream);
-    if (pieces <= 1024 * 16) return launch_row<T, 1024, 16>(a, two, stream);
-    return launch_row<T, 1024, 0>(a, two, stream);
+    if (!a.grad) {
+        if (pieces <= 64 * 8) return launch_row<T, 64, 0, false>(a, stream);
+        return launch_row<T, 512, 0, false>(a, stream);
+    }
+    if (pieces <= 64 * 8) return launch_row<T, 64, 8, true>(a, stream);
+    if (pieces <= 256 * 8) return launch_row<T, 256, 8, true>(a, stream);
+    if (pieces <= 512 * 8) return launch_row<T, 512, 8, true>(a, stream);
+    if (pieces <= 512 * 16) return launch_row<T, 512, 16, true>(a, stream);
+    return launch_row<T, 512, 0, true>(a, stream);
 }
 }  // namespace
 
@@ -397,9 +621,9 @@ size_t distillation_workspace(const gscan_rows &rows) {
     return kCountBlocks * sizeof(int) + (size_t)part_blocks(rows) * 3 * sizeof(double);
 }
 
-int distillation_loss(const gscan_rows &rows, const gscan_distillation &t, const float *upstream, void *grad, float *stats,
-                      void *workspace, size_t bytes, hipStream_t stream) {
-    GSCAN_CHECK(stats, "distillation_loss: stats is NULL");
+int distillation_loss(const gscan_rows &rows, const gscan_distillation &t, const float *upstream, void *grad, float *loss,
+                      float *stats, void *workspace, size_t bytes, hipStream_t stream) {
+    GSCAN_CHECK(loss || (grad && !stats), "distillation_loss: loss is NULL");
     GSCAN_CHECK(t.K >= 1 && t.K <= kMaxTop, "distillation_loss: %d teacher entries per row (1 to %d)", t.K, kMaxTop);
     GSCAN_CHECK(t.indices && t.teacher, "distillation_loss: the teacher's indices or logits are NULL");
     GSCAN_CHECK(t.index_bits == 32 || t.index_bits == 64, "distillation_loss: %d bits per index (32 or 64)", t.index_bits);
@@ -422,19 +646,24 @@ int distillation_loss(const gscan_rows &rows, const gscan_distillation &t, const
     a.labels = t.labels; a.ignore = t.ignore_index; a.shift = t.shift_labels != 0;
     a.inv_tau = 1.f / t.temperature;
     a.soft = t.soft_weight; a.soft_grad = t.soft_weight * t.temperature; a.hard = t.hard_weight;
+    a.power = t.temperature == 2.f ? 2 : t.temperature == 3.f ? 3 : t.temperature == 4.f ? 4 : 0;
     a.upstream = upstream; a.grad = (char *)grad;
+    a.far = (int64_t)a.count * rows.V * b >= kFarGradient;
     a.part = (double *)(live + kCountBlocks);
-    if (grad && !t.sum_reduction) {       // the gradient of a mean needs the number of live rows first
+    a.sum = t.sum_reduction != 0;
+    if (grad && !a.sum && a.count > (rows.V <= 64 ? kCountThere : kCountThereLong)) {       // the gradient of a mean needs the number of live rows first
         a.live = live;
         hipLaunchKernelGGL(distill_count_kernel, dim3(kCountBlocks), dim3(256), 0, stream, a, live);
         GSCAN_LAUNCHED("distill_count_kernel");
     }
     const int type = rows.type;
-    TRY_RC(type == GSCAN_F32 ? launch_type<TypeF32>(a, stream) : type == GSCAN_BF16 ? launch_type<TypeBF16>(a, stream)
-                                                                                   : launch_type<TypeF16>(a, stream));
+    TRY_RC(type == GSCAN_F32    ? launch_type<TypeF32>(a, stream)
+           : type == GSCAN_BF16 ? launch_type<TypeBF16>(a, stream)
+                                : launch_type<TypeF16>(a, stream));
+    if (!loss) return 0;
     const float tau2 = t.temperature * t.temperature;
     hipLaunchKernelGGL(distill_finish_kernel, dim3(1), dim3(1024), 0, stream, a.part, part_blocks(rows), t.soft_weight * tau2,
-                       t.hard_weight, t.sum_reduction ? 0 : 1, stats);
+                       t.hard_weight, t.sum_reduction ? 0 : 1, loss, stats);
     GSCAN_LAUNCHED("distill_finish_kernel");
     return 0;
 }

@@ -19,8 +19,8 @@ size_t top_logits_workspace(const gscan_rows &rows, int K);
 int top_logits(const gscan_rows &rows, int K, void *values, int32_t *indices, float *lse, void *workspace, size_t bytes,
                hipStream_t stream);
 size_t distillation_workspace(const gscan_rows &rows);
-int distillation_loss(const gscan_rows &rows, const gscan_distillation &terms, const float *upstream, void *grad, float *stats,
-                      void *workspace, size_t bytes, hipStream_t stream);
+int distillation_loss(const gscan_rows &rows, const gscan_distillation &terms, const float *upstream, void *grad, float *loss,
+                      float *stats, void *workspace, size_t bytes, hipStream_t stream);
 size_t beam_select_workspace(const gscan_rows &rows);
 int beam_select(const gscan_rows &rows, const float *scores, const uint8_t *finished, int eos, int pad, float *scores_out,
                 int32_t *parents, int64_t *tokens, uint8_t *finished_out, void *workspace, size_t bytes, hipStream_t stream);
@@ -61,28 +61,30 @@ static inline Rows device_rows(const gscan_rows &r) {
 
 struct Raw { uint32_t w[4]; };    // 16 bytes of a row
 
-template <class T>
+typedef uint32_t Quad2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t Quad4 __attribute__((ext_vector_type(4), aligned(4)));
+
+template <class T, bool STREAM = false>
 __device__ __forceinline__ Raw load16(const char *p) {
-    Raw r;
-    if constexpr (T::bytes == 4) {
-        struct __attribute__((packed, aligned(4))) U { uint32_t w[4]; };
-        const U u = *(const U *)p;
-        r.w[0] = u.w[0]; r.w[1] = u.w[1]; r.w[2] = u.w[2]; r.w[3] = u.w[3];
+    Quad2 q;
+    if constexpr (STREAM) {
+        if constexpr (T::bytes == 4) q = __builtin_nontemporal_load((const Quad4 *)p);
+        else q = __builtin_nontemporal_load((const Quad2 *)p);
     } else {
-        struct __attribute__((packed, aligned(2))) U { uint32_t w[4]; };
-        const U u = *(const U *)p;
-        r.w[0] = u.w[0]; r.w[1] = u.w[1]; r.w[2] = u.w[2]; r.w[3] = u.w[3];
+        if constexpr (T::bytes == 4) q = *(const Quad4 *)p;
+        else q = *(const Quad2 *)p;
     }
-    return r;
+    return Raw{{q.x, q.y, q.z, q.w}};
 }
-template <class T>
+template <class T, bool STREAM = false>
 __device__ __forceinline__ void store16(char *p, const Raw &r) {
+    const Quad2 q = {r.w[0], r.w[1], r.w[2], r.w[3]};
     if constexpr (T::bytes == 4) {
-        struct __attribute__((packed, aligned(4))) U { uint32_t w[4]; };
-        *(U *)p = U{{r.w[0], r.w[1], r.w[2], r.w[3]}};
+        if constexpr (STREAM) __builtin_nontemporal_store((Quad4)q, (Quad4 *)p);
+        else *(Quad4 *)p = q;
     } else {
-        struct __attribute__((packed, aligned(2))) U { uint32_t w[4]; };
-        *(U *)p = U{{r.w[0], r.w[1], r.w[2], r.w[3]}};
+        if constexpr (STREAM) __builtin_nontemporal_store(q, (Quad2 *)p);
+        else *(Quad2 *)p = q;
     }
 }
 
@@ -180,26 +182,46 @@ __device__ __forceinline__ V wave_reduce(V v, Op op) {
     return v;
 }
 
+// log sum exp from the parts of a row's chunks, in 64 bits; one wave.
+__device__ __forceinline__ double join_lse(const LsePart *part, int n) {
+    const int lane = threadIdx.x & 63;
+    float ref = -FLT_MAX;
+    for (int i = lane; i < n; i += 64) ref = fmaxf(ref, part[i].ref);
+    ref = wave_reduce(ref, [](float a, float b) { return fmaxf(a, b); });
+    double s = 0.0;
+    for (int i = lane; i < n; i += 64) s += part[i].sum * exp((double)part[i].ref - (double)ref);
+    s = wave_reduce(s, [](double a, double b) { return a + b; });
+    return ref == INFINITY ? (double)INFINITY : (double)ref + log(s);
+}
+
 // A number t such that at least K of n keys in LDS are >= t, and (unless many are equal) few more than K: bisection between
 // the keys' least and largest, counting with ballots; it ends as soon as the count is within K .. K + K/4, or the interval is
 // one number.  One wave, n <= 64 * SLOTS.  With fewer than K keys > 0 the answer is 0.
 template <int SLOTS>
 __device__ __forceinline__ uint32_t kth_bound(const uint32_t *keys, int n, int K, int lane) {
-    uint32_t k[SLOTS], hi = 0;
+    uint32_t k[SLOTS], hi = 0, lo = ~0u;
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i) {
         k[i] = lane + 64 * i < n ? keys[lane + 64 * i] : 0u;
-        hi = k[i] > hi ? k[i] : hi;
+        hi = max(hi, k[i]);
+        if (k[i]) lo = min(lo, k[i]);
     }
-    hi = __builtin_amdgcn_readfirstlane(wave_reduce(hi, [](uint32_t a, uint32_t b) { return a > b ? a : b; }));
-    uint32_t lo = 0;            // count(>= lo) >= K (0: all of them) holds throughout; count(>= hi + 1) = 0 < K
-    uint64_t top = (uint64_t)hi + 1;
-    const int most = K + (K >> 2);
-    while (top - lo > 1) {
-        const uint32_t mid = (uint32_t)(lo + (top - lo) / 2);
+    auto count = [&](uint32_t least) {
         int c = 0;
 #pragma unroll
-        for (int i = 0; i < SLOTS; ++i) c += __popcll(__ballot(k[i] >= mid));
+        for (int i = 0; i < SLOTS; ++i) c += __popcll(__ballot(k[i] >= least));
+        return c;
+    };
+    if (count(1) < K) return 0;
+    // count(>= lo) >= K and count(>= top) < K throughout; a lane's largest key bounds from below too where K <= 64 lanes
+    const uint32_t least = K <= 64 && __ballot(hi != 0) == ~0ull ? hi : lo;
+    lo = __builtin_amdgcn_readfirstlane(wave_reduce(least, [](uint32_t a, uint32_t b) { return min(a, b); }));
+    hi = __builtin_amdgcn_readfirstlane(wave_reduce(hi, [](uint32_t a, uint32_t b) { return max(a, b); }));
+    const int most = K + (K >> 2);
+    uint32_t top = hi + 1;       // keys of numbers end far below 2^32 - 1
+    while (top - lo > 1) {
+        const uint32_t mid = lo + (top - lo) / 2;
+        const int c = count(mid);
         if (c >= K) {
             lo = mid;
             if (c <= most) break;

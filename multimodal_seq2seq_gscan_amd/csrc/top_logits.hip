@@ -8,6 +8,8 @@
 // (little more than K words unless many are equal) is ranked in LDS by counting.  Exact for any input: where the words >= the
 // bound do not fit the list, words above it and, in index order, words equal to it are taken apart, and if even the words
 // above it do not fit (a row laid out against this grouping), a radix selection over the row finds the K-th key.
+#include <cstddef>
+
 #include "logits.h"
 
 namespace gscan {
@@ -52,8 +54,9 @@ struct EntrySource {
 
 template <int TPB>
 struct TopShared {
-    uint64_t cand[kCap];
+    alignas(16) uint64_t cand[kCap + 2];
     uint32_t keys[4 * TPB];         // the groups' maxima; the radix selection's histogram
+    uint32_t thread_keys[TPB];
     uint16_t hit[4 * TPB];          // groups to read again
     uint32_t bound;
     int hits, count, above;
@@ -154,25 +157,40 @@ __device__ int radix_select(const S &src, TopShared<TPB> &sh, int K, uint32_t *k
     return need;
 }
 
-// With the groups' maxima in sh.keys: leaves candidates that hold the K best entries in sh.cand and returns their number.
-template <int TPB, class S>
-__device__ int find_candidates(const S &src, TopShared<TPB> &sh, int K) {
-    const int tid = threadIdx.x, G = 4 * TPB;
+// With the groups' maxima in sh.keys (and, for a small K, the threads' maxima over their four groups in sh.thread_keys):
+// leaves candidates that hold the K best entries in sh.cand and returns their number.  `scan(bound)` puts the entries >= bound
+// on the list without reading again, where it can.
+template <int TPB, class S, class F>
+__device__ int find_candidates(const S &src, TopShared<TPB> &sh, int K, F scan) {
+    constexpr int G = 4 * TPB;
+    const int tid = threadIdx.x;
     __syncthreads();
     if (tid < 64) {
-        const uint32_t b = kth_bound<4 * TPB / 64>(sh.keys, G, K, tid);
+        // K of TPB threads' maxima bound nearly as well as K of four times as many, for a quarter of the counting, while K is
+        // no more than a quarter of them
+        const uint32_t b = 4 * K <= TPB ? kth_bound<TPB / 64>(sh.thread_keys, TPB, K, tid) : kth_bound<G / 64>(sh.keys, G, K, tid);
         if (tid == 0) { sh.bound = b; sh.hits = 0; sh.count = 0; }
     }
     __syncthreads();
     const uint32_t bound = sh.bound;
+    if constexpr (!__is_same(F, std::nullptr_t)) {
+        scan(bound);
+        __syncthreads();
+        if (sh.count <= kCap) return sh.count;
+        __syncthreads();
+        if (tid == 0) sh.count = 0;
+    }
     for (int g = tid; g < G; g += TPB)
         if (sh.keys[g] >= bound && sh.keys[g]) sh.hit[atomicAdd(&sh.hits, 1)] = (uint16_t)g;
     __syncthreads();
-    int n = collect<TPB>(src, sh, bound, true);
-    if (n <= kCap) return n;
-    __syncthreads();
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
+    int n;
+    if constexpr (__is_same(F, std::nullptr_t)) {
+        n = collect<TPB>(src, sh, bound, true);
+        if (n <= kCap) return n;
+        __syncthreads();
+        if (tid == 0) sh.count = 0;
+        __syncthreads();
+    }
     n = collect<TPB>(src, sh, bound, false);
     if (n >= K && n <= kCap) return n;
     if (n < K) {
@@ -194,10 +212,17 @@ __device__ int find_candidates(const S &src, TopShared<TPB> &sh, int K) {
 // Every candidate's place is the number of candidates before it; `put(place, entry)` for the first K of them.
 template <int TPB, class F>
 __device__ __forceinline__ void rank_candidates(TopShared<TPB> &sh, int n, int K, F put) {
+    const int even = (n + 1) & ~1;
+    if (threadIdx.x == 0 && even > n) sh.cand[n] = 0;
+    __syncthreads();
     for (int i = threadIdx.x; i < n; i += TPB) {
         const uint64_t x = sh.cand[i];
         int place = 0;
-        for (int j = 0; j < n; ++j) place += sh.cand[j] > x ? 1 : 0;
+#pragma unroll 4
+        for (int j = 0; j < even; j += 2) {
+            const ulonglong2 q = *(const ulonglong2 *)&sh.cand[j];
+            place += (q.x > x ? 1 : 0) + (q.y > x ? 1 : 0);
+        }
         if (place < K) put(place, x);
     }
 }
@@ -208,8 +233,9 @@ __device__ __forceinline__ void put_out(const TopArgs &a, int64_t at, uint64_t x
     a.indices[at] = (int32_t)~(uint32_t)x;
 }
 
-// One workgroup per row, or per chunk of a row.
-template <class T, int TPB, bool LSE>
+// One workgroup per row, or per chunk of a row.  HELD: a row (chunk) of at most four pieces a thread, which stay in registers:
+// nothing is read again.
+template <class T, int TPB, bool LSE, bool HELD>
 __global__ __launch_bounds__(TPB) void top_row_kernel(TopArgs a) {
     __shared__ TopShared<TPB> sh;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -233,28 +259,50 @@ __global__ __launch_bounds__(TPB) void top_row_kernel(TopArgs a) {
         const float m = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), ref);
         if (m > ref) { sum *= __builtin_amdgcn_exp2f((ref - m) * kLog2e); ref = m; }
     };
-    int p = tid;
-    for (; p + 3 * TPB < full; p += 4 * TPB) {
-        Raw x[4];
+    Raw held[HELD ? 4 : 1];
+    if constexpr (HELD) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) x[u] = load16<T>(base + (int64_t)(p + u * TPB) * 16);
+        for (int u = 0; u < 4; ++u)
+            if (tid + u * TPB < pieces) held[u] = src.load(tid + u * TPB);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) take(x[u], top[u]);
+        for (int u = 0; u < 4; ++u)
+            if (tid + u * TPB < pieces) take(held[u], top[u]);
         if constexpr (LSE) {
             rescale();
 #pragma unroll
-            for (int u = 0; u < 4; ++u) add(x[u]);
+            for (int u = 0; u < 4; ++u)
+                if (tid + u * TPB < pieces) add(held[u]);
         }
+    } else {
+        int p = tid;
+        for (; p + 3 * TPB < full; p += 4 * TPB) {
+            Raw x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] = load16<T>(base + (int64_t)(p + u * TPB) * 16);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) take(x[u], top[u]);
+            if constexpr (LSE) {
+                rescale();
+#pragma unroll
+                for (int u = 0; u < 4; ++u) add(x[u]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (p + u * TPB < pieces) {
+                const Raw x = src.load(p + u * TPB);
+                take(x, top[u]);
+                if constexpr (LSE) { rescale(); add(x); }
+            }
     }
+    uint32_t most = 0;
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-        if (p + u * TPB < pieces) {
-            const Raw x = src.load(p + u * TPB);
-            take(x, top[u]);
-            if constexpr (LSE) { rescale(); add(x); }
-        }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) sh.keys[u * TPB + tid] = tid + u * TPB < pieces ? order_key(top[u]) : 0u;
+    for (int u = 0; u < 4; ++u) {
+        const uint32_t k = tid + u * TPB < pieces ? order_key(top[u]) : 0u;
+        sh.keys[u * TPB + tid] = k;
+        most = max(most, k);
+    }
+    sh.thread_keys[tid] = most;
 
     if constexpr (LSE) {
         const float m = wave_reduce(ref, [](float x, float y) { return fmaxf(x, y); });
@@ -273,7 +321,25 @@ __global__ __launch_bounds__(TPB) void top_row_kernel(TopArgs a) {
             else a.lse[r] = all == INFINITY ? INFINITY : (float)((double)all + log(s));
         }
     }
-    const int n = find_candidates<TPB>(src, sh, a.K);
+    int n;
+    if constexpr (HELD) {
+        n = find_candidates<TPB>(src, sh, a.K, [&](uint32_t bound) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (sh.keys[u * TPB + tid] >= bound && tid + u * TPB < pieces) {
+#pragma unroll
+                    for (int e = 0; e < T::vec; ++e) {
+                        const uint64_t x = src.entry(held[u], tid + u * TPB, e);
+                        if (x && (uint32_t)(x >> 32) >= bound) {
+                            const int at = atomicAdd(&sh.count, 1);
+                            if (at < kCap) sh.cand[at] = x;
+                        }
+                    }
+                }
+        });
+    } else {
+        n = find_candidates<TPB>(src, sh, a.K, nullptr);
+    }
     __syncthreads();
     if (a.keys) {
         uint64_t *out = a.keys + (int64_t)blockIdx.x * a.K;
@@ -298,17 +364,14 @@ __global__ __launch_bounds__(TPB) void top_join_kernel(TopArgs a) {
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) sh.keys[u * TPB + tid] = top[u];
-    const int n = find_candidates<TPB>(src, sh, a.K);
+    sh.thread_keys[tid] = max(max(top[0], top[1]), max(top[2], top[3]));
+    if (a.lse && tid >= TPB - 64) {        // the last wave: the first one looks for the bound
+        const double total = join_lse(a.parts + (int64_t)r * a.splits, a.splits);
+        if (tid == TPB - 1) a.lse[r] = (float)total;
+    }
+    const int n = find_candidates<TPB>(src, sh, a.K, nullptr);
     __syncthreads();
     rank_candidates<TPB>(sh, n, a.K, [&](int place, uint64_t x) { put_out<T>(a, (int64_t)r * a.K + place, x); });
-    if (a.lse && tid == 0) {
-        const LsePart *part = a.parts + (int64_t)r * a.splits;
-        float ref = part[0].ref;
-        for (int i = 1; i < a.splits; ++i) ref = fmaxf(ref, part[i].ref);
-        double s = 0.0;
-        for (int i = 0; i < a.splits; ++i) s += part[i].sum * exp((double)part[i].ref - (double)ref);
-        a.lse[r] = ref == INFINITY ? INFINITY : (float)((double)ref + log(s));
-    }
 }
 
 // Vocabularies of at most 64 words: L lanes per row, a word per lane, a word's place counted against the other lanes'.
@@ -336,14 +399,20 @@ __global__ __launch_bounds__(256) void top_small_kernel(TopArgs a, int rows) {
 // A wave per row where a wave's 256 groups suffice for K and a row is short: no barrier is waited at.
 bool one_wave(const gscan_rows &rows, int K) { return K <= 64 && rows.V <= 2048; }
 
-template <class T>
-int launch_rows(const TopArgs &a, int64_t grid, bool lse, bool wave, hipStream_t stream) {
-    if (wave && lse) hipLaunchKernelGGL((top_row_kernel<T, 64, true>), dim3((unsigned)grid), dim3(64), 0, stream, a);
-    else if (wave) hipLaunchKernelGGL((top_row_kernel<T, 64, false>), dim3((unsigned)grid), dim3(64), 0, stream, a);
-    else if (lse) hipLaunchKernelGGL((top_row_kernel<T, 256, true>), dim3((unsigned)grid), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((top_row_kernel<T, 256, false>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+template <class T, int TPB>
+int launch_rows(const TopArgs &a, int64_t grid, bool lse, hipStream_t stream) {
+    const dim3 blocks((unsigned)grid);
+    const bool held = a.chunk <= 4 * TPB * T::vec;
+    if (lse && held) hipLaunchKernelGGL((top_row_kernel<T, TPB, true, true>), blocks, dim3(TPB), 0, stream, a);
+    else if (lse) hipLaunchKernelGGL((top_row_kernel<T, TPB, true, false>), blocks, dim3(TPB), 0, stream, a);
+    else if (held) hipLaunchKernelGGL((top_row_kernel<T, TPB, false, true>), blocks, dim3(TPB), 0, stream, a);
+    else hipLaunchKernelGGL((top_row_kernel<T, TPB, false, false>), blocks, dim3(TPB), 0, stream, a);
     GSCAN_LAUNCHED("top_row_kernel");
     return 0;
+}
+template <class T>
+int launch_rows(const TopArgs &a, int64_t grid, bool lse, bool wave, hipStream_t stream) {
+    return wave ? launch_rows<T, 64>(a, grid, lse, stream) : launch_rows<T, 256>(a, grid, lse, stream);
 }
 
 template <class T>

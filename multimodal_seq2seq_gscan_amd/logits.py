@@ -10,6 +10,7 @@ this package."""
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -20,26 +21,30 @@ _TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _li
 _INDEX_BITS = {torch.int32: 32, torch.int64: 64}
 
 
-def _require(device: torch.device, **tensors: torch.Tensor) -> None:
-    for name, t in tensors.items():
+def _require(names: str, *tensors: Optional[torch.Tensor]) -> int:
+    """The index of the device that all of the tensors are on; raises for a CPU tensor or two devices."""
+    index = tensors[0].get_device()
+    for i, t in enumerate(tensors):
         if t is None:
             continue
         if not t.is_cuda:
-            raise RuntimeError(f"{name} is on {t.device}: this operator runs on the HIP device only (there is no CPU fallback "
-                               "in this package)")
-        if t.device != device:
-            raise ValueError(f"{name} is on {t.device}, the other tensors are on {device}")
+            raise RuntimeError(f"{names.split()[i]} is on {t.device}: this operator runs on the HIP device only (there is no CPU "
+                               "fallback in this package)")
+        if t.get_device() != index:
+            raise ValueError(f"{names.split()[i]} is on {t.device}, {names.split()[0]} is on {tensors[0].device}")
+    return index
 
 
-def _call(name: str, device: torch.device, *args) -> None:
+def _call(name: str, device: int, *args) -> None:
     """One library call on the current stream of `device`, with that device current."""
     fn = getattr(_lib.load(), name)
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if device == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(rc, name)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _float_type(t: torch.Tensor, name: str) -> int:
@@ -86,18 +91,18 @@ def top_logits(logits: torch.Tensor, k: int, return_lse: bool = False) -> Tuple[
 
     Value descending, the lowest index first among equals.  A NaN counts as -inf, and is returned as -inf.
     1 <= k <= min(V, 256).  No gradient flows through it."""
-    _require(logits.device, logits=logits)
-    logits, rows = _rows(logits.detach())
+    device = _require("logits", logits)
+    logits, rows = _rows(logits)
     k = int(k)
     if not 1 <= k <= min(rows.V, _lib.MAX_TOP):
         raise ValueError(f"k must be 1 to {min(rows.V, _lib.MAX_TOP)} for rows of {rows.V} words, got {k}")
-    lead, device = logits.shape[:-1], logits.device
-    values = torch.empty(*lead, k, dtype=logits.dtype, device=device)
-    indices = torch.empty(*lead, k, dtype=torch.int32, device=device)
-    lse = torch.empty(lead, dtype=torch.float32, device=device) if return_lse else None
+    lead, where = logits.shape[:-1], logits.device
+    values = torch.empty(*lead, k, dtype=logits.dtype, device=where)
+    indices = torch.empty(*lead, k, dtype=torch.int32, device=where)
+    lse = torch.empty(lead, dtype=torch.float32, device=where) if return_lse else None
     if values.numel():
         size = _lib.load().gscan_top_logits_workspace_bytes(C.byref(rows), k)
-        ws = _workspace(size, device)
+        ws = _workspace(size, where)
         _call("gscan_top_logits", device, C.byref(rows), k, values.data_ptr(), indices.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), size)
     return (values, indices, lse) if return_lse else (values, indices)
 
@@ -107,9 +112,9 @@ def top_logits(logits: torch.Tensor, k: int, return_lse: bool = False) -> Tuple[
 # ---------------------------------------------------------------------------------------------------------------------
 def _distillation(logits, teacher_indices, teacher_logits, labels, temperature, soft_weight, hard_weight, ignore_index,
                   shift_labels, reduction):
-    """Checks the arguments; (logits, rows, terms, tensors that the terms point at)."""
-    _require(logits.device, logits=logits, teacher_indices=teacher_indices, teacher_logits=teacher_logits, labels=labels)
-    logits, rows = _rows(logits.detach())
+    """Checks the arguments; (device, logits, rows, terms, tensors that the terms point at)."""
+    device = _require("logits teacher_indices teacher_logits labels", logits, teacher_indices, teacher_logits, labels)
+    logits, rows = _rows(logits)
     lead = logits.shape[:-1]
     if teacher_indices.dtype not in _INDEX_BITS:
         raise TypeError(f"teacher_indices must be int32 or int64, got {teacher_indices.dtype}")
@@ -135,44 +140,45 @@ def _distillation(logits, teacher_indices, teacher_logits, labels, temperature, 
             raise TypeError(f"labels must be int64, got {labels.dtype}")
         if labels.shape != lead:
             raise ValueError(f"labels must be {tuple(lead)}, got {tuple(labels.shape)}")
-        labels = labels.detach().contiguous()
-    indices, teacher = teacher_indices.detach().contiguous(), teacher_logits.detach().contiguous()
+        labels = labels.contiguous()
+    indices, teacher = teacher_indices.contiguous(), teacher_logits.contiguous()
     terms = _lib.Distillation(indices.data_ptr(), teacher.data_ptr(), _lib.ptr(labels), int(ignore_index),
                               _INDEX_BITS[indices.dtype], kind, K, int(bool(shift_labels)), temperature, soft_weight, hard_weight,
                               int(reduction == "sum"))
-    return logits, rows, terms, (indices, teacher, labels)
+    return device, logits, rows, terms, (indices, teacher, labels)
 
 
-def _launch_distillation(logits, rows, terms, upstream: Optional[torch.Tensor], grad: Optional[torch.Tensor],
-                         stats: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """stats [4]: sum of the hard losses, live rows, sum of the divergences, loss."""
-    device = logits.device
+def _launch_distillation(device: int, logits, rows, terms, upstream: Optional[torch.Tensor], grad: Optional[torch.Tensor],
+                         stats: Optional[torch.Tensor] = None, want_loss: bool = True) -> Optional[torch.Tensor]:
+    """The loss (None where only the gradient is wanted); `stats` [4] receives [sum of the rows' losses, live rows, sum of the hard terms, sum of the divergences]."""
+    where = logits.device
     if logits.numel() == 0:
-        return torch.zeros(4, dtype=torch.float32, device=device) if stats is None else stats.zero_()
-    if stats is None:
-        stats = torch.empty(4, dtype=torch.float32, device=device)
+        if stats is not None:
+            stats.zero_()
+        return torch.zeros((), dtype=torch.float32, device=where)
+    loss = torch.empty((), dtype=torch.float32, device=where) if want_loss else None
     size = _lib.load().gscan_distillation_workspace_bytes(C.byref(rows))
-    ws = _workspace(size, device)
-    _call("gscan_distillation_loss", device, C.byref(rows), C.byref(terms), _lib.ptr(upstream), _lib.ptr(grad), stats.data_ptr(),
-          _lib.ptr(ws), size)
-    return stats
+    ws = torch.empty(size, dtype=torch.uint8, device=where)
+    _call("gscan_distillation_loss", device, C.byref(rows), C.byref(terms), _lib.ptr(upstream), _lib.ptr(grad), _lib.ptr(loss),
+          _lib.ptr(stats), ws.data_ptr(), size)
+    return loss
 
 
 class _DistillationLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, indices, teacher, labels, options):
-        logits, rows, terms, kept = _distillation(logits, indices, teacher, labels, *options)
+        device, logits, rows, terms, kept = _distillation(logits, indices, teacher, labels, *options)
         ctx.save_for_backward(logits, *kept)
         ctx.options = options
-        return _launch_distillation(logits, rows, terms, None, None)[3]
+        return _launch_distillation(device, logits, rows, terms, None, None)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         logits, indices, teacher, labels = ctx.saved_tensors
-        logits, rows, terms, _ = _distillation(logits, indices, teacher, labels, *ctx.options)
+        device, logits, rows, terms, _ = _distillation(logits, indices, teacher, labels, *ctx.options)
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        _launch_distillation(logits, rows, terms, g.to(torch.float32).contiguous(), grad)
+        _launch_distillation(device, logits, rows, terms, g.to(torch.float32).contiguous(), grad, want_loss=False)
         return grad, None, None, None, None
 
 
@@ -195,8 +201,8 @@ def distillation_loss(logits: torch.Tensor, teacher_indices: torch.Tensor, teach
     options = (temperature, soft_weight, hard_weight, ignore_index, shift_labels, reduction)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _DistillationLoss.apply(logits, teacher_indices, teacher_logits, labels, options)
-    logits, rows, terms, _kept = _distillation(logits, teacher_indices, teacher_logits, labels, *options)
-    return _launch_distillation(logits, rows, terms, None, None)[3]
+    device, logits, rows, terms, _kept = _distillation(logits, teacher_indices, teacher_logits, labels, *options)
+    return _launch_distillation(device, logits, rows, terms, None, None)
 
 
 def distillation_loss_and_gradient(logits: torch.Tensor, teacher_indices: torch.Tensor, teacher_logits: torch.Tensor,
@@ -206,21 +212,21 @@ def distillation_loss_and_gradient(logits: torch.Tensor, teacher_indices: torch.
     """`distillation_loss` and its gradient with respect to the logits in one pass over them, outside autograd: what a loop
     that issues its own backward pass calls (`train.TrainStep`).  Returns (loss, gradient [..., V] of the logits' type);
     `out`: a contiguous tensor for the gradient, which may not share memory with the logits."""
-    logits, rows, terms, _kept = _distillation(logits, teacher_indices, teacher_logits, labels, temperature, soft_weight, hard_weight,
-                                        ignore_index, shift_labels, reduction)
-    out = _gradient_out(logits, out)
-    return _launch_distillation(logits, rows, terms, None, out)[3], out
-
-
-def _gradient_out(logits: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
+    device, logits, rows, terms, _kept = _distillation(logits, teacher_indices, teacher_logits, labels, temperature, soft_weight,
+                                                       hard_weight, ignore_index, shift_labels, reduction)
     if out is None:
-        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    _require(logits.device, out=out)
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    else:
+        _check_gradient_out(logits, out)
+    return _launch_distillation(device, logits, rows, terms, None, out), out
+
+
+def _check_gradient_out(logits: torch.Tensor, out: torch.Tensor) -> None:
+    _require("logits out", logits, out)
     if out.shape != logits.shape or out.dtype != logits.dtype or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {tuple(logits.shape)} tensor of {logits.dtype}")
     if _overlap(out, logits):
         raise ValueError("out shares memory with the logits")
-    return out
 
 
 def _extent(t: torch.Tensor) -> Tuple[int, int]:
@@ -247,10 +253,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
     (scores [B, W], parents [B, W] int32, words [B, W] int64, finished [B, W] bool: the parent was, or the word is `eos_idx`).
     Start a search with scores of 0 for one beam and -inf for the others: beams of -inf fill only places that nothing else
     takes.  W <= 64, V <= 2^24; a word barred with -inf (or NaN) has the score -inf."""
-    _require(logits.device, logits=logits, scores=scores, finished=finished)
+    device = _require("logits scores finished", logits, scores, finished)
     if logits.dim() != 3:
         raise ValueError(f"logits must be [B, W, V], got {tuple(logits.shape)}")
-    logits, rows = _rows(logits.detach())
+    logits, rows = _rows(logits)
     B, W, V = logits.shape
     if tuple(scores.shape) != (B, W) or tuple(finished.shape) != (B, W):
         raise ValueError(f"scores and finished must be [{B}, {W}], got {tuple(scores.shape)} and {tuple(finished.shape)}")
@@ -260,15 +266,15 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
         raise ValueError(f"1 to {_lib.MAX_BEAMS} beams and at most 2^24 words, got {W} and {V}")
     if not (0 <= int(eos_idx) < V and 0 <= int(pad_idx) < V):
         raise ValueError(f"eos_idx {eos_idx} or pad_idx {pad_idx} is not one of the {V} words")
-    device = logits.device
-    scores, finished = scores.detach().contiguous(), finished.contiguous()
-    new_scores = torch.empty(B, W, dtype=torch.float32, device=device)
-    parents = torch.empty(B, W, dtype=torch.int32, device=device)
-    words = torch.empty(B, W, dtype=torch.int64, device=device)
-    done = torch.empty(B, W, dtype=torch.bool, device=device)
+    where = logits.device
+    scores, finished = scores.contiguous(), finished.contiguous()
+    new_scores = torch.empty(B, W, dtype=torch.float32, device=where)
+    parents = torch.empty(B, W, dtype=torch.int32, device=where)
+    words = torch.empty(B, W, dtype=torch.int64, device=where)
+    done = torch.empty(B, W, dtype=torch.bool, device=where)
     if B:
         size = _lib.load().gscan_beam_select_workspace_bytes(C.byref(rows))
-        ws = _workspace(size, device)
+        ws = _workspace(size, where)
         _call("gscan_beam_select", device, C.byref(rows), scores.data_ptr(), finished.data_ptr(), int(eos_idx), int(pad_idx),
               new_scores.data_ptr(), parents.data_ptr(), words.data_ptr(), done.data_ptr(), _lib.ptr(ws), size)
     return new_scores, parents, words, done
@@ -307,6 +313,12 @@ def _slices(src: torch.Tensor, dst: torch.Tensor, dim: int) -> Optional[_lib.Sta
                       dims[dim][1] * size, dims[dim][2] * size, mid[1] * size, mid[2] * size)
 
 
+@functools.lru_cache(maxsize=None)
+def _table(n: int):
+    """The array type of n states (ctypes makes a new class for every `State * n`)."""
+    return _lib.State * n
+
+
 def beam_reorder(parents: torch.Tensor, states: Union[torch.Tensor, Sequence[torch.Tensor]],
                  out: Union[None, torch.Tensor, Sequence[torch.Tensor]] = None, dim: int = 0
                  ) -> Union[torch.Tensor, List[torch.Tensor]]:
@@ -319,18 +331,17 @@ def beam_reorder(parents: torch.Tensor, states: Union[torch.Tensor, Sequence[tor
     sources = [states] if single else list(states)
     if parents.dim() != 2 or parents.dtype != torch.int32:
         raise ValueError(f"parents must be an int32 tensor [B, W], got {parents.dtype} {tuple(parents.shape)}")
-    device = parents.device
-    _require(device, parents=parents)
+    device = _require("parents", parents)
     B, W = parents.shape
     if out is None:
-        targets = [torch.empty(s.shape, dtype=s.dtype, device=s.device) for s in sources]
+        targets = [torch.empty(s.shape, dtype=s.dtype, device=parents.device) for s in sources]
     else:
         targets = [out] if isinstance(out, torch.Tensor) else list(out)
         if len(targets) != len(sources):
             raise ValueError(f"{len(sources)} states, but {len(targets)} tensors to write them to")
     moves = []
     for i, (s, d) in enumerate(zip(sources, targets)):
-        _require(device, **{f"states[{i}]": s, f"out[{i}]": d})
+        _require(f"parents states[{i}] out[{i}]", parents, s, d)
         at = dim + s.dim() if dim < 0 else dim
         if not 0 <= at < s.dim() or s.shape[at] != B * W:
             raise ValueError(f"states[{i}] {tuple(s.shape)} has not {B} x {W} entries along dimension {dim}")
@@ -340,7 +351,6 @@ def beam_reorder(parents: torch.Tensor, states: Union[torch.Tensor, Sequence[tor
             continue
         if out is not None and any(_overlap(d, other) for other in sources):
             raise ValueError(f"out[{i}] shares memory with a state")
-        s = s.detach()
         move = _slices(s, d, at)
         if move is None:
             s = s.contiguous()
@@ -354,7 +364,7 @@ def beam_reorder(parents: torch.Tensor, states: Union[torch.Tensor, Sequence[tor
             spans = sorted(_extent(d) for d in targets if d.numel())
             if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
                 raise ValueError("two tensors of out share memory")
-        table = (_lib.State * len(moves))(*(m for m, _ in moves))
+        table = _table(len(moves))(*(m for m, _ in moves))
         order = parents.contiguous()
         _call("gscan_beam_reorder", device, B, W, order.data_ptr(), table, len(moves))
     return targets[0] if single else targets

@@ -197,10 +197,11 @@ def test_distillation_matches_its_formula(ops, dtype, lead, V, K, options):
     weight = kw.get("soft_weight", 1.0) * kw.get("temperature", 1.0) ** 2 + kw.get("hard_weight", 0.0)
     check_loss(loss, want, rows * weight * (2 + math.log(V)))
     check_gradient(got, grad, size, dtype)
-    assert torch.equal(ops.distillation_loss(zd, idd, td, yd, **kw), loss)
+    alone = ops.distillation_loss(zd, idd, td, yd, **kw)      # without the gradient a row's sums are taken in another order
+    check_loss(alone, want, rows * weight * (2 + math.log(V)))
     leaf = zd.clone().requires_grad_()
     up = ops.distillation_loss(leaf, idd, td, yd, **kw)
-    assert up.requires_grad and torch.equal(up.detach(), loss)
+    assert up.requires_grad and torch.equal(up.detach(), alone)
     (up * -2.5).backward()
     check_gradient(leaf.grad, grad * -2.5, size * 2.5, dtype)
     assert torch.equal(ops.distillation_loss_and_gradient(zd, idd, td, yd, **kw)[1], got)       # the same bits again

@@ -18,7 +18,7 @@ def lib():
 def on_host(monkeypatch, lib):
     """The Python layer with CPU tensors and no launches: its checks only."""
     calls = []
-    monkeypatch.setattr(ops, "_require", lambda device, **tensors: None)
+    monkeypatch.setattr(ops, "_require", lambda names, *tensors: 0)
     monkeypatch.setattr(ops, "_call", lambda name, device, *args: calls.append(name))
     return calls
 
@@ -72,16 +72,16 @@ def terms(**kw):
                                      (dict(hard_weight=float("inf")), "weights"), (dict(hard_weight=float("nan")), "weights"),
                                      (dict(labels=None), "labels")])
 def test_library_refuses_bad_distillation(lib, kw, word):
-    assert lib.gscan_distillation_loss(C.byref(rows()), C.byref(terms(**kw)), None, None, 4096, 4096, 1 << 20, None) != 0
+    assert lib.gscan_distillation_loss(C.byref(rows()), C.byref(terms(**kw)), None, None, 4096, None, 4096, 1 << 20, None) != 0
     assert word in message(lib)
 
 
 def test_library_refuses_missing_outputs_and_small_workspaces(lib):
-    assert lib.gscan_distillation_loss(C.byref(rows()), C.byref(terms()), None, None, None, 4096, 1 << 20, None) != 0
+    assert lib.gscan_distillation_loss(C.byref(rows()), C.byref(terms()), None, None, None, None, 4096, 1 << 20, None) != 0
     need = lib.gscan_distillation_workspace_bytes(C.byref(rows()))
-    assert lib.gscan_distillation_loss(C.byref(rows()), C.byref(terms()), None, None, 4096, 4096, need - 1, None) != 0
+    assert lib.gscan_distillation_loss(C.byref(rows()), C.byref(terms()), None, None, 4096, None, 4096, need - 1, None) != 0
     assert "workspace" in message(lib)
-    assert lib.gscan_distillation_loss(C.byref(rows()), None, None, None, 4096, 4096, need, None) != 0
+    assert lib.gscan_distillation_loss(C.byref(rows()), None, None, None, 4096, None, 4096, need, None) != 0
     select = [C.byref(rows(inner=4)), 4096, 4096, 2, 0, 8192, 8192, 8192, 8192, None, 0, None]
     assert lib.gscan_beam_select(*select) != 0 and "workspace" in message(lib)
     for at, bad, word in ((1, None, "NULL"), (3, 100, "eos"), (4, -1, "pad"), (5, 4096, "inputs")):
