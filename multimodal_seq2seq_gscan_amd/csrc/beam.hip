@@ -69,7 +69,7 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamArgs a) {
             if (c == 0) { key = order_key64(-INFINITY); v = (uint32_t)k; }
         } else {
             const uint64_t x = i == tid ? early : keys[i];
-            if (x) { key = score_key((double)score, (double)key_value((uint32_t)(x >> 32)), s_lse[w]); v = ~(uint32_t)x; }
+            if (x) { key = score_key((double)score, (double)key_value(pair_value(x)), s_lse[w]); v = (uint32_t)pair_index(x); }
         }
         s_key[i] = key;
         s_flat[i] = (uint32_t)w * (uint32_t)a.rows.V + v;
@@ -181,7 +181,7 @@ BeamPlan beam_plan(const gscan_rows &rows) {
 
 // ---- reordering ----
 constexpr int kMaxStates = 16;           // per launch: the table travels in the kernel's arguments
-constexpr int kSegment = 8192;           // bytes that a wave copies
+constexpr int kSegment = 4096;           // bytes that a wave copies
 constexpr int64_t kMaxItems = 1 << 28;   // pieces of one state: a launch's blocks stay below 2^31
 
 struct CopyState {
@@ -191,20 +191,35 @@ struct CopyState {
 };
 struct CopyArgs { int B, W, count; const int32_t *parents; CopyState s[kMaxStates]; };
 
+// The table's pointers are global memory; told so, the copies are global instructions and not flat ones.
 template <class U>
 __device__ __forceinline__ void copy_segment(const char *in, char *out, int n, int lane, bool zero) {
+    typedef const __attribute__((address_space(1))) U *In;
+    typedef __attribute__((address_space(1))) U *Out;
+    constexpr int R = kSegment / 16 / 64;
     const int words = n / (int)sizeof(U);
-    int i = lane;
-    for (; i + 7 * 64 < words; i += 8 * 64) {
-        U x[8];
+    const In src = (In)(uintptr_t)in + lane;
+    const Out dst = (Out)(uintptr_t)out + lane;
+    int i = 0;
+    for (; i + R * 64 <= words; i += R * 64) {
+        U x[R];
+        if (zero) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) x[u] = zero ? U{} : ((const U *)in)[i + u * 64];
+            for (int u = 0; u < R; ++u) x[u] = U{};
+        } else {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) ((U *)out)[i + u * 64] = x[u];
+            for (int u = 0; u < R; ++u) x[u] = src[i + u * 64];
+        }
+#pragma unroll
+        for (int u = 0; u < R; ++u) dst[i + u * 64] = x[u];
     }
-    for (; i < words; i += 64) ((U *)out)[i] = zero ? U{} : ((const U *)in)[i];
+    for (; i + lane < words; i += 64) dst[i] = zero ? U{} : src[i];
 }
 
+// A wave per segment of a slice, its four loads before its four stores.  The bytes bind it: 1.07 GB of states written (and
+// what of as much is read: parents repeat) in 285 us, where a plain copy of them takes 400 and writing zeros 192.  A wave per
+// batch row's segments that reads a parent once for all of its children is slower (307): repeated readings come from the last
+// cache.  Segments of 8 KB: 289.
 __global__ __launch_bounds__(256) void beam_reorder_kernel(CopyArgs a) {
     int k = 0;
     while (k + 1 < a.count && (int)blockIdx.x >= a.s[k + 1].first_block) ++k;
@@ -217,7 +232,7 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(CopyArgs a) {
     const int m = q % s.mid;
     q /= s.mid;
     const int row = q % rows, o = q / rows, b = row / a.W;
-    const int parent = a.parents[row];
+    const int parent = __builtin_amdgcn_readfirstlane(a.parents[row]);
     const bool zero = parent < 0 || parent >= a.W;       // nothing is read for it
     const int64_t at = (int64_t)seg * kSegment;
     const char *in = s.in + o * s.in_outer + (int64_t)(b * a.W + (zero ? 0 : parent)) * s.in_row + m * s.in_mid + at;

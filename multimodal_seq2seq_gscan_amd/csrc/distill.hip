@@ -23,10 +23,6 @@ constexpr int kCountBlocks = 64;
 // less: 22.8 for 27.1 us at 5120 rows of 9 words); longer rows fill the chip with workgroups, and theirs come from a launch
 // before them (4088 rows of 32000 words: 134 for 152 us).
 constexpr int kCountThere = 8192, kCountThereLong = 256;
-// Gradients from so many bytes on are stored past the caches (non-temporal), as they leave the 256 MB of the last one before
-// anything reads them: 262 MB 125 -> 115 us; 131 MB would go from 73 to 76.
-constexpr int64_t kFarGradient = 192 << 20;
-
 struct DistillArgs {
     Rows rows;
     int count;                         // rows in all
@@ -41,7 +37,6 @@ struct DistillArgs {
     const int *live;                   // kCountBlocks partial counts of the live rows, or NULL: counted where they are needed
     const float *upstream;             // or NULL: 1
     char *grad;                        // [rows][V], or NULL
-    int far;                           // stored past the caches
     double *part;                      // [workgroups][3]: hard loss, soft loss, live rows
 };
 
@@ -244,10 +239,7 @@ __global__ __launch_bounds__(TPB) __attribute__((amdgpu_waves_per_eu(4))) void d
     const int r = blockIdx.x, label = row_label(a, r);
     double *part = a.part + 3 * (int64_t)r;
     char *out = GRAD ? a.grad + (int64_t)r * V * T::bytes : nullptr;
-    auto store = [&](char *to, const Raw &w) {
-        if (NR == 0 || a.far) store16<T, true>(to, w);
-        else store16<T>(to, w);
-    };
+    auto store = [&](char *to, const Raw &w) { store16<T, NR == 0>(to, w); };
     if (label == -1) {                 // not live: neither its words nor its teacher's are read
         if constexpr (GRAD) {
             for (int p = tid; p < pieces; p += TPB) store(out + (int64_t)p * 16, Raw{{0, 0, 0, 0}});
@@ -648,7 +640,6 @@ int distillation_loss(const gscan_rows &rows, const gscan_distillation &t, const
     a.soft = t.soft_weight; a.soft_grad = t.soft_weight * t.temperature; a.hard = t.hard_weight;
     a.power = t.temperature == 2.f ? 2 : t.temperature == 3.f ? 3 : t.temperature == 4.f ? 4 : 0;
     a.upstream = upstream; a.grad = (char *)grad;
-    a.far = (int64_t)a.count * rows.V * b >= kFarGradient;
     a.part = (double *)(live + kCountBlocks);
     a.sum = t.sum_reduction != 0;
     if (grad && !a.sum && a.count > (rows.V <= 64 ? kCountThere : kCountThereLong)) {       // the gradient of a mean needs the number of live rows first

@@ -172,8 +172,13 @@ __device__ __forceinline__ uint64_t order_key64(double d) {
     const uint64_t u = (uint64_t)__double_as_longlong(d + 0.0);
     return u ^ ((uint64_t)((int64_t)u >> 63) | 0x8000000000000000ull);
 }
-// (value, index) as one number: larger = earlier in the order (value descending, index ascending)
-__device__ __forceinline__ uint64_t pair_key(uint32_t key, int index) { return ((uint64_t)key << 32) | (uint32_t)~index; }
+// (value, index) as one number: larger = earlier in the order (value descending, index ascending); 0 = no entry.  62 bits, an
+// index being below 2^30: also as a double's bits the numbers are in order (positive, finite), and two doubles are compared at
+// several times the rate of two 64-bit integers.
+__device__ __forceinline__ uint64_t pair_key(uint32_t key, int index) { return ((uint64_t)key << 30) | (0x3fffffffu - (uint32_t)index); }
+__device__ __forceinline__ uint32_t pair_value(uint64_t x) { return (uint32_t)(x >> 30); }
+__device__ __forceinline__ int pair_index(uint64_t x) { return (int)(0x3fffffffu - ((uint32_t)x & 0x3fffffffu)); }
+__device__ __forceinline__ double pair_double(uint64_t x) { return __longlong_as_double((int64_t)x); }
 
 template <typename V, class Op>
 __device__ __forceinline__ V wave_reduce(V v, Op op) {

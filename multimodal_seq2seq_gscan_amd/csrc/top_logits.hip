@@ -2,12 +2,15 @@
 // (distill.hip) and what a beam search looks at in a step (beam.hip).  Order: value descending, index ascending; a NaN counts
 // as -inf.
 //
-// One pass over the row, then a few per mille of it a second time: 4 TPB groups of a row's 16-byte pieces keep one maximum
-// each.  At least K words are >= the K-th largest of these maxima, so it bounds the K-th largest word from below, and a group
-// whose maximum is below the bound holds none of the K: only the other groups' pieces are read again, and what is >= the bound
-// (little more than K words unless many are equal) is ranked in LDS by counting.  Exact for any input: where the words >= the
-// bound do not fit the list, words above it and, in index order, words equal to it are taken apart, and if even the words
-// above it do not fit (a row laid out against this grouping), a radix selection over the row finds the K-th key.
+// One pass over the row.  Every thread keeps the maximum of the words that it has seen (four maxima for a large K); at least K
+// words are >= the K-th largest of these maxima, so it bounds the K-th largest word from below.  LDS holds 16 bits of the
+// maximum of every 16-byte piece: the few pieces that reach the bound are read again, their words >= the bound (little more
+// than K unless many are equal) are ranked by counting.  Without the pieces' maxima a thread's whole share of the row would be
+// read again for every thread above the bound, a 128-byte line for every 16 bytes: 68 against 57 us for 4088 rows of 32000
+// bfloat16 words, K = 64.
+// Exact for any input: where the words >= the bound do not fit the list, words above it and, in index order, words equal to
+// it are taken apart, and if even the words above it do not fit (a row laid out against the threads), a radix selection over
+// the row finds the K-th key.
 #include <cstddef>
 
 #include "logits.h"
@@ -15,7 +18,7 @@
 namespace gscan {
 
 namespace {
-constexpr int kCap = 1024;         // candidates in LDS: at least 4 kMaxTop
+constexpr int kHits = 1024;        // groups of pieces that reach the bound
 
 struct TopArgs {
     Rows rows;
@@ -25,14 +28,29 @@ struct TopArgs {
     const uint8_t *finished; const float *scores;    // beam step: a row that is finished or has no score is left out
 };
 
+// What is looked for: entries whose key is > `key`, or >= it.
+struct Limit {
+    uint32_t key;
+    bool equal;
+    float value;          // of the key, and whether every word reaches it
+    bool all;
+    __device__ __forceinline__ Limit(uint32_t k, bool eq) : key(k), equal(eq), value(key_value(k)), all(eq && k <= 0x007fffffu) {}
+};
+
 // Words of a row (or of a part of it), 16 bytes at a time.
 template <class T>
 struct WordSource {
     static constexpr int vec = T::vec;
+    typedef Raw Piece;
     const char *row;      // of the whole row
     int first, n;         // the part: words [first, first + n), first a multiple of vec
     __device__ __forceinline__ int pieces() const { return (n + vec - 1) / vec; }
     __device__ __forceinline__ Raw load(int p) const { return load_group<T>(row + (int64_t)first * T::bytes, p, n); }
+    // (a NaN is below every limit but that of -inf)
+    __device__ __forceinline__ bool reaches(const Raw &r, int p, int e, const Limit &l) const {
+        const float z = element<T>(r, e);
+        return (l.all || z > l.value || (l.equal && z == l.value)) && p * vec + e < n;
+    }
     __device__ __forceinline__ uint64_t entry(const Raw &r, int p, int e) const {       // 0: behind the end
         const int i = p * vec + e;
         return i < n ? pair_key(order_key(element<T>(r, e)), first + i) : 0ull;
@@ -44,20 +62,32 @@ struct WordSource {
 // Entries that chunks of a row have left, one at a time (0: none).
 struct EntrySource {
     static constexpr int vec = 1;
+    typedef uint64_t Piece;
     const uint64_t *list;
     int n;
     __device__ __forceinline__ int pieces() const { return n; }
     __device__ __forceinline__ uint64_t load(int p) const { return list[p]; }
+    __device__ __forceinline__ bool reaches(uint64_t r, int, int, const Limit &l) const {
+        const uint32_t k = pair_value(r);
+        return k > l.key || (l.equal && k == l.key && k);
+    }
     __device__ __forceinline__ uint64_t entry(uint64_t r, int, int) const { return r; }
     __device__ __forceinline__ uint64_t at(int i) const { return list[i]; }
 };
 
-template <int TPB>
+// PIECES: how many pieces' (or groups of pieces') maxima are held, 0 for none.
+template <int TPB, int PIECES>
 struct TopShared {
-    alignas(16) uint64_t cand[kCap + 2];
-    uint32_t keys[4 * TPB];         // the groups' maxima; the radix selection's histogram
+    // candidates: at least 4 K (a wave takes K <= 64); pieces that reach the bound, where they need not be read again
+    static constexpr int kCap = TPB == 64 ? 512 : 1024, kStash = TPB == 64 ? 256 : 512;
+    union {
+        alignas(16) uint64_t cand[kCap + 2];
+        uint32_t keys[4 * TPB];         // four maxima a thread, until there is a bound; the radix selection's histogram
+    };
     uint32_t thread_keys[TPB];
-    uint16_t hit[4 * TPB];          // groups to read again
+    alignas(16) uint16_t piece[PIECES ? PIECES : 1];
+    alignas(16) Raw stash[PIECES ? 1 : kStash];
+    uint16_t hit[PIECES ? kHits : kStash];
     uint32_t bound;
     int hits, count, above;
     int wave_count[TPB / 64];
@@ -65,40 +95,59 @@ struct TopShared {
     float ref[TPB / 64];
 };
 
-// Reads the pieces of the groups on the list again and puts the entries whose key is > bound (or >= it) on the list of
-// candidates; returns how many there are, which may be more than fit.
-template <int TPB, class S>
-__device__ __forceinline__ int collect(const S &src, TopShared<TPB> &sh, uint32_t bound, bool equal) {
-    const int tid = threadIdx.x, hits = sh.hits, pieces = src.pieces();
-    const int per = (pieces + 4 * TPB - 1) / (4 * TPB);
-    const int items = hits * per;
-    for (int it = tid; it < items; it += TPB) {
-        const int h = it / per, p = sh.hit[h] + (it - h * per) * (4 * TPB);
-        if (p >= pieces) continue;
-        const auto raw = src.load(p);
+// The thread's number with the waves turned round by the workgroup's: what few waves of a workgroup do falls on another of the
+// CU's four SIMDs from one workgroup to the next.
+template <int TPB>
+__device__ __forceinline__ int turned() { return (int)((threadIdx.x + 64 * blockIdx.x) & (TPB - 1)); }
+
+// Place for `total` entries (the same in every lane) behind a list's; one atomic a wave.
+__device__ __forceinline__ int reserve(int *count, int total) {
+    int at = 0;
+    if ((threadIdx.x & 63) == 0) at = atomicAdd(count, total);
+    return __builtin_amdgcn_readfirstlane(at);
+}
+__device__ __forceinline__ int lanes_before(unsigned long long mask) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
+}
+// Puts the entries of a piece a lane that reach the limit on the list of candidates; every lane of a wave takes part, one
+// without a piece with p behind the last.  What does not fit is counted only.
+template <class S, class Sh>
+__device__ __forceinline__ void push_piece(const S &src, Sh &sh, const typename S::Piece &raw, int p, const Limit &l) {
+    unsigned long long b[S::vec];
+    int total = 0;
 #pragma unroll
-        for (int e = 0; e < S::vec; ++e) {
-            const uint64_t x = src.entry(raw, p, e);
-            const uint32_t k = (uint32_t)(x >> 32);
-            if (k > bound || (equal && k == bound && k)) {
-                const int at = atomicAdd(&sh.count, 1);
-                if (at < kCap) sh.cand[at] = x;
-            }
-        }
+    for (int e = 0; e < S::vec; ++e) {
+        b[e] = __ballot(p < src.pieces() && src.reaches(raw, p, e, l));
+        total += __popcll(b[e]);
     }
-    __syncthreads();
-    return sh.count;
+    if (total == 0) return;
+    int at = reserve(&sh.count, total);
+#pragma unroll
+    for (int e = 0; e < S::vec; ++e) {
+        if (b[e] == 0) continue;
+        const int mine = at + lanes_before(b[e]);
+        if ((b[e] >> (threadIdx.x & 63) & 1) && mine < Sh::kCap) sh.cand[mine] = src.entry(raw, p, e);
+        at += __popcll(b[e]);
+    }
+}
+template <int TPB, class S, class Sh>
+__device__ __forceinline__ void scan_all(const S &src, Sh &sh, uint32_t bound, bool equal) {
+    const Limit l(bound, equal);
+    for (int base = 0; base < src.pieces(); base += TPB) {
+        const int p = base + (int)threadIdx.x;
+        push_piece(src, sh, src.load(min(p, src.pieces() - 1)), p, l);
+    }
 }
 
 // The first `want` entries, in index order, whose key is `key`, behind the `at` candidates that are there.
-template <int TPB, class S>
-__device__ void collect_equal(const S &src, TopShared<TPB> &sh, uint32_t key, int at, int want) {
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, words = src.pieces() * S::vec;
+template <int TPB, class S, class Sh>
+__device__ void collect_equal(const S &src, Sh &sh, uint32_t key, int at, int want) {
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     int found = 0;
-    for (int base = 0; base < words && found < want; base += TPB) {
+    for (int base = 0; base < src.n && found < want; base += TPB) {
         const int i = base + tid;
         const uint64_t x = i < src.n ? src.at(i) : 0ull;
-        const bool is = x && (uint32_t)(x >> 32) == key;
+        const bool is = x && pair_value(x) == key;
         const unsigned long long b = __ballot(is);
         if (lane == 0) sh.wave_count[wave] = __popcll(b);
         __syncthreads();
@@ -116,8 +165,8 @@ __device__ void collect_equal(const S &src, TopShared<TPB> &sh, uint32_t key, in
 
 // The K-th largest key of the whole source by radix selection (eight bits a pass); returns how many entries equal to it
 // belong to the K.  Entered with more than K entries.
-template <int TPB, class S>
-__device__ int radix_select(const S &src, TopShared<TPB> &sh, int K, uint32_t *key) {
+template <int TPB, class S, class Sh>
+__device__ int radix_select(const S &src, Sh &sh, int K, uint32_t *key) {
     const int tid = threadIdx.x, pieces = src.pieces();
     uint32_t prefix = 0;
     int need = K;
@@ -128,7 +177,7 @@ __device__ int radix_select(const S &src, TopShared<TPB> &sh, int K, uint32_t *k
             const auto raw = src.load(p);
 #pragma unroll
             for (int e = 0; e < S::vec; ++e) {
-                const uint32_t k = (uint32_t)(src.entry(raw, p, e) >> 32);
+                const uint32_t k = pair_value(src.entry(raw, p, e));
                 if (k && (shift == 24 || (k >> (shift + 8)) == prefix)) atomicAdd(&sh.keys[(k >> shift) & 255], 1u);
             }
         }
@@ -157,42 +206,35 @@ __device__ int radix_select(const S &src, TopShared<TPB> &sh, int K, uint32_t *k
     return need;
 }
 
-// With the groups' maxima in sh.keys (and, for a small K, the threads' maxima over their four groups in sh.thread_keys):
-// leaves candidates that hold the K best entries in sh.cand and returns their number.  `scan(bound)` puts the entries >= bound
-// on the list without reading again, where it can.
-template <int TPB, class S, class F>
-__device__ int find_candidates(const S &src, TopShared<TPB> &sh, int K, F scan) {
-    constexpr int G = 4 * TPB;
-    const int tid = threadIdx.x;
+// With the threads' maxima in sh.thread_keys (and four a thread in sh.keys): leaves candidates that hold the K best entries in
+// sh.cand and returns their number.  `scan(bound)` puts the entries >= bound on the list; it may leave some out where it
+// counts more than fit.
+template <int TPB, class S, class Sh, class F>
+__device__ int find_candidates(const S &src, Sh &sh, int K, F scan) {
+    const int tid = turned<TPB>();
     __syncthreads();
     if (tid < 64) {
-        // K of TPB threads' maxima bound nearly as well as K of four times as many, for a quarter of the counting, while K is
-        // no more than a quarter of them
-        const uint32_t b = 4 * K <= TPB ? kth_bound<TPB / 64>(sh.thread_keys, TPB, K, tid) : kth_bound<G / 64>(sh.keys, G, K, tid);
+        // K of TPB maxima bound nearly as well as K of four times as many, for a quarter of the counting, while K is no more
+        // than a quarter of them
+        const uint32_t b = 4 * K <= TPB ? kth_bound<TPB / 64>(sh.thread_keys, TPB, K, tid) : kth_bound<4 * TPB / 64>(sh.keys, 4 * TPB, K, tid);
         if (tid == 0) { sh.bound = b; sh.hits = 0; sh.count = 0; }
     }
     __syncthreads();
     const uint32_t bound = sh.bound;
-    if constexpr (!__is_same(F, std::nullptr_t)) {
-        scan(bound);
-        __syncthreads();
-        if (sh.count <= kCap) return sh.count;
-        __syncthreads();
-        if (tid == 0) sh.count = 0;
-    }
-    for (int g = tid; g < G; g += TPB)
-        if (sh.keys[g] >= bound && sh.keys[g]) sh.hit[atomicAdd(&sh.hits, 1)] = (uint16_t)g;
+    scan(bound);
     __syncthreads();
-    int n;
-    if constexpr (__is_same(F, std::nullptr_t)) {
-        n = collect<TPB>(src, sh, bound, true);
-        if (n <= kCap) return n;
+    int n = sh.count;
+    if (n <= Sh::kCap) return n;
+    auto again = [&](uint32_t key) {
         __syncthreads();
         if (tid == 0) sh.count = 0;
         __syncthreads();
-    }
-    n = collect<TPB>(src, sh, bound, false);
-    if (n >= K && n <= kCap) return n;
+        scan_all<TPB>(src, sh, key, false);
+        __syncthreads();
+        return sh.count;
+    };
+    n = again(bound);
+    if (n >= K && n <= Sh::kCap) return n;
     if (n < K) {
         collect_equal<TPB>(src, sh, bound, n, K - n);
         return K;
@@ -200,44 +242,79 @@ __device__ int find_candidates(const S &src, TopShared<TPB> &sh, int K, F scan) 
     __syncthreads();
     uint32_t key;
     const int equal = radix_select<TPB>(src, sh, K, &key);
-    // every group may hold entries above the K-th key: all of them are read again
-    if (tid == 0) { sh.hits = G; sh.count = 0; }
-    for (int g = tid; g < G; g += TPB) sh.hit[g] = (uint16_t)g;
-    __syncthreads();
-    n = collect<TPB>(src, sh, key, false);
+    n = again(key);
     collect_equal<TPB>(src, sh, key, n, equal);
     return K;
 }
 
 // Every candidate's place is the number of candidates before it; `put(place, entry)` for the first K of them.
-template <int TPB, class F>
-__device__ __forceinline__ void rank_candidates(TopShared<TPB> &sh, int n, int K, F put) {
+template <int TPB, class Sh, class F>
+__device__ __forceinline__ void rank_candidates(Sh &sh, int n, int K, F put) {
     const int even = (n + 1) & ~1;
+    __syncthreads();
     if (threadIdx.x == 0 && even > n) sh.cand[n] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += TPB) {
+    for (int i = turned<TPB>(); i < n; i += TPB) {
         const uint64_t x = sh.cand[i];
+        const double mine = pair_double(x);
         int place = 0;
 #pragma unroll 4
         for (int j = 0; j < even; j += 2) {
-            const ulonglong2 q = *(const ulonglong2 *)&sh.cand[j];
-            place += (q.x > x ? 1 : 0) + (q.y > x ? 1 : 0);
+            const double2 q = *(const double2 *)&sh.cand[j];
+            place += (q.x > mine ? 1 : 0) + (q.y > mine ? 1 : 0);
         }
         if (place < K) put(place, x);
     }
 }
 
+// A thread's sum exp(z - ref) over the words so far.  Near 0 as 2^(z log2 e + back), back = -ref log2 e rounded: one
+// multiply-add a word; the sum is off by the factor 2^delta, delta = what the rounding added, which is known and is taken off
+// when the reference changes and at the end (candidates of different beams are compared through this sum: 32 bits of it are
+// not given away).  Far out, where delta grows, the distance from the reference comes first.
+struct RunningSum {
+    float sum = 0.f, ref = -FLT_MAX, back = 0.f, delta = 0.f;
+    bool near = false;
+    __device__ __forceinline__ void clear() { sum = 0.f; }
+    __device__ __forceinline__ void grow(float m) {
+        if (m > ref) {
+            const bool n = fabsf(m) < 65536.f;
+            const float b = n ? -m * kLog2e : 0.f, d = n ? fmaf(m, kLog2e, b) : 0.f;
+            sum *= __builtin_amdgcn_exp2f((ref - m) * kLog2e + (d - delta));
+            ref = m; back = b; delta = d; near = n;
+        }
+    }
+    template <int N>
+    __device__ __forceinline__ void add(const float (&z)[N]) {
+        if (near) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum += __builtin_amdgcn_exp2f(fmaf(z[e], kLog2e, back));
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum += __builtin_amdgcn_exp2f((z[e] - ref) * kLog2e);
+        }
+    }
+    __device__ __forceinline__ void add_word(float z) {
+        const float one[1] = {z};
+        add(one);
+    }
+    __device__ __forceinline__ double relative_to(float m) const {
+        // 2^-delta to the first order: delta is below 2^-7
+        const double d = (double)delta * 0.6931471805599453;
+        return (double)sum * (1.0 - d + 0.5 * d * d) * (double)__builtin_amdgcn_exp2f((ref - m) * kLog2e);
+    }
+};
+
 template <class T>
 __device__ __forceinline__ void put_out(const TopArgs &a, int64_t at, uint64_t x) {
-    store1<T>((char *)a.values, at, key_value((uint32_t)(x >> 32)));
-    a.indices[at] = (int32_t)~(uint32_t)x;
+    store1<T>((char *)a.values, at, key_value(pair_value(x)));
+    a.indices[at] = pair_index(x);
 }
 
-// One workgroup per row, or per chunk of a row.  HELD: a row (chunk) of at most four pieces a thread, which stay in registers:
-// nothing is read again.
-template <class T, int TPB, bool LSE, bool HELD>
+// One workgroup per row, or per chunk of a row.  PIECES = 0: at most four pieces a thread, which stay in registers: nothing is
+// read again.
+template <class T, int TPB, bool LSE, int PIECES>
 __global__ __launch_bounds__(TPB) void top_row_kernel(TopArgs a) {
-    __shared__ TopShared<TPB> sh;
+    __shared__ TopShared<TPB, PIECES> sh;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int r = blockIdx.x / a.splits, c = blockIdx.x - r * a.splits;
     if (a.finished && (a.finished[r] || a.scores[r] == -INFINITY)) return;
@@ -246,27 +323,30 @@ __global__ __launch_bounds__(TPB) void top_row_kernel(TopArgs a) {
     const char *base = src.row + (int64_t)src.first * T::bytes;
 
     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    float ref = -FLT_MAX, sum = 0.f;      // sum exp(z - ref) so far
-    auto take = [&](const Raw &x, float &t) {
+    RunningSum sum;
+    auto largest = [&](const Raw &x) {
+        float t = element<T>(x, 0);
 #pragma unroll
-        for (int e = 0; e < T::vec; ++e) t = fmaxf(t, element<T>(x, e));
+        for (int e = 1; e < T::vec; ++e) t = fmaxf(t, element<T>(x, e));
+        return fmaxf(t, -INFINITY);
     };
+    auto rescale = [&]() { sum.grow(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))); };
     auto add = [&](const Raw &x) {
+        float z[T::vec];
 #pragma unroll
-        for (int e = 0; e < T::vec; ++e) sum += __builtin_amdgcn_exp2f((fmaxf(element<T>(x, e), -INFINITY) - ref) * kLog2e);
+        for (int e = 0; e < T::vec; ++e) z[e] = element<T>(x, e);
+        sum.add(z);
     };
-    auto rescale = [&]() {
-        const float m = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), ref);
-        if (m > ref) { sum *= __builtin_amdgcn_exp2f((ref - m) * kLog2e); ref = m; }
-    };
-    Raw held[HELD ? 4 : 1];
-    if constexpr (HELD) {
+    Raw held[PIECES ? 1 : 4];
+    // group (s, t) of pieces: t + TPB (per s + k), k < per
+    const int steps = (pieces + TPB - 1) / TPB, per = PIECES ? max(1, (steps + PIECES / TPB - 1) / (PIECES / TPB)) : 1;
+    if constexpr (PIECES == 0) {
 #pragma unroll
         for (int u = 0; u < 4; ++u)
             if (tid + u * TPB < pieces) held[u] = src.load(tid + u * TPB);
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-            if (tid + u * TPB < pieces) take(held[u], top[u]);
+            if (tid + u * TPB < pieces) top[u] = largest(held[u]);
         if constexpr (LSE) {
             rescale();
 #pragma unroll
@@ -274,17 +354,30 @@ __global__ __launch_bounds__(TPB) void top_row_kernel(TopArgs a) {
                 if (tid + u * TPB < pieces) add(held[u]);
         }
     } else {
+        float group = -INFINITY;
+        int s = 0, k = 0;
+        auto take = [&](const Raw &x, float &t) {
+            const float m = largest(x);
+            t = fmaxf(t, m);
+            group = fmaxf(group, m);
+            if (++k == per) {
+                sh.piece[s * TPB + tid] = (uint16_t)(order_key(group) >> 16);
+                group = -INFINITY; k = 0; ++s;
+            }
+        };
         int p = tid;
         for (; p + 3 * TPB < full; p += 4 * TPB) {
             Raw x[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) x[u] = load16<T>(base + (int64_t)(p + u * TPB) * 16);
+            for (int u = 0; u < 4; ++u) x[u] = load16<T, true>(base + (int64_t)(p + u * TPB) * 16);
 #pragma unroll
             for (int u = 0; u < 4; ++u) take(x[u], top[u]);
             if constexpr (LSE) {
                 rescale();
+                float z[4 * T::vec];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) add(x[u]);
+                for (int i = 0; i < 4 * T::vec; ++i) z[i] = element<T>(x[i / T::vec], i % T::vec);
+                sum.add(z);
             }
         }
 #pragma unroll
@@ -294,53 +387,117 @@ __global__ __launch_bounds__(TPB) void top_row_kernel(TopArgs a) {
                 take(x, top[u]);
                 if constexpr (LSE) { rescale(); add(x); }
             }
+        // a group that is not full, and those that this thread has no piece of
+        const int groups = (steps + per - 1) / per;
+        if (k) { sh.piece[s * TPB + tid] = (uint16_t)(order_key(group) >> 16); ++s; }
+        for (; s < groups; ++s) sh.piece[s * TPB + tid] = 0;
     }
     uint32_t most = 0;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
         const uint32_t k = tid + u * TPB < pieces ? order_key(top[u]) : 0u;
-        sh.keys[u * TPB + tid] = k;
+        if (4 * a.K > TPB) sh.keys[u * TPB + tid] = k;
         most = max(most, k);
     }
     sh.thread_keys[tid] = most;
 
     if constexpr (LSE) {
-        const float m = wave_reduce(ref, [](float x, float y) { return fmaxf(x, y); });
+        if (sum.sum != sum.sum) {          // a NaN among the words (or an infinity): they count as -inf
+            sum.clear();
+            for (int p = tid; p < pieces; p += TPB) {
+                const Raw x = src.load(p);
+#pragma unroll
+                for (int e = 0; e < T::vec; ++e) sum.add_word(fmaxf(element<T>(x, e), -INFINITY));
+            }
+        }
+        const float m = wave_max(sum.ref);
         if (lane == 0) sh.ref[wave] = m;
         __syncthreads();
         float all = sh.ref[0];
         for (int w = 1; w < TPB / 64; ++w) all = fmaxf(all, sh.ref[w]);
-        double s = (double)sum * (double)__builtin_amdgcn_exp2f((ref - all) * kLog2e);
+        double s = sum.relative_to(all);
         s = wave_reduce(s, [](double x, double y) { return x + y; });
         if (lane == 0) sh.sum[wave] = s;
         __syncthreads();
-        if (tid == 0) {
+        if (tid == TPB - 1) {          // not of the wave that looks for the bound
             s = sh.sum[0];
             for (int w = 1; w < TPB / 64; ++w) s += sh.sum[w];
             if (a.parts) a.parts[blockIdx.x] = LsePart{s, all, 0.f};
             else a.lse[r] = all == INFINITY ? INFINITY : (float)((double)all + log(s));
         }
     }
-    int n;
-    if constexpr (HELD) {
-        n = find_candidates<TPB>(src, sh, a.K, [&](uint32_t bound) {
+    const int n = find_candidates<TPB>(src, sh, a.K, [&](uint32_t bound) {
+        const Limit l(bound, true);
+        if constexpr (PIECES == 0) {
+            // a lane in sixteen holds such a piece: they are dealt out to a lane each before their words are looked at
+            unsigned long long m[4];
+            int total = 0;
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (sh.keys[u * TPB + tid] >= bound && tid + u * TPB < pieces) {
+            for (int u = 0; u < 4; ++u) {
+                m[u] = __ballot(tid + u * TPB < pieces && (l.all || top[u] >= l.value));
+                total += __popcll(m[u]);
+            }
+            if (total) {
+                int at = reserve(&sh.hits, total);
 #pragma unroll
-                    for (int e = 0; e < T::vec; ++e) {
-                        const uint64_t x = src.entry(held[u], tid + u * TPB, e);
-                        if (x && (uint32_t)(x >> 32) >= bound) {
-                            const int at = atomicAdd(&sh.count, 1);
-                            if (at < kCap) sh.cand[at] = x;
-                        }
-                    }
+                for (int u = 0; u < 4; ++u) {
+                    const int mine = at + lanes_before(m[u]);
+                    if ((m[u] >> lane & 1) && mine < sh.kStash) { sh.stash[mine] = held[u]; sh.hit[mine] = (uint16_t)(tid + u * TPB); }
+                    at += __popcll(m[u]);
                 }
-        });
-    } else {
-        n = find_candidates<TPB>(src, sh, a.K, nullptr);
-    }
-    __syncthreads();
+            }
+            __syncthreads();
+            const int hits = sh.hits;
+            if (hits > sh.kStash) {                   // (nearly) all words alike: the caller goes over the row
+                if (tid == 0) sh.count = sh.kCap + 1;
+                return;
+            }
+            for (int it = turned<TPB>(); (it & ~63) < hits; it += TPB) {
+                const int at = min(it, sh.kStash - 1);
+                push_piece(src, sh, sh.stash[at], it < hits ? (int)sh.hit[at] : pieces, l);
+            }
+        } else {
+            const int groups = (steps + per - 1) / per * TPB;
+            const uint32_t least = max(bound >> 16, 1u);
+            constexpr int pairs = PIECES / TPB / 2;      // two groups' maxima at a time
+            uint32_t two[pairs];
+            int total = 0;
+#pragma unroll
+            for (int i = 0; i < pairs; ++i) {
+                const int g = 2 * (tid + i * TPB);
+                two[i] = g < groups ? *(const uint32_t *)&sh.piece[g] : 0u;
+                total += __popcll(__ballot((two[i] & 0xffffu) >= least)) + __popcll(__ballot((two[i] >> 16) >= least));
+            }
+            if (total) {
+                int at = reserve(&sh.hits, total);
+#pragma unroll
+                for (int i = 0; i < pairs; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const bool hit = (h ? two[i] >> 16 : two[i] & 0xffffu) >= least;
+                        const unsigned long long m = __ballot(hit);
+                        if (m == 0) continue;
+                        const int mine = at + lanes_before(m);
+                        if (hit && mine < kHits) sh.hit[mine] = (uint16_t)(2 * (tid + i * TPB) + h);
+                        at += __popcll(m);
+                    }
+            }
+            __syncthreads();
+            const int hits = sh.hits, items = hits * per;
+            if (hits > kHits) {                    // (nearly) all words alike: the caller goes over the row
+                if (tid == 0) sh.count = sh.kCap + 1;
+                return;
+            }
+            for (int it = turned<TPB>(); (it & ~63) < items; it += TPB) {
+                int p = pieces;
+                if (it < items) {
+                    const int h = it / per, g = sh.hit[h];
+                    p = (g & (TPB - 1)) + TPB * (per * (g / TPB) + it - h * per);
+                }
+                push_piece(src, sh, src.load(min(p, pieces - 1)), p, l);
+            }
+        }
+    });
     if (a.keys) {
         uint64_t *out = a.keys + (int64_t)blockIdx.x * a.K;
         rank_candidates<TPB>(sh, n, a.K, [&](int place, uint64_t x) { out[place] = x; });
@@ -353,14 +510,14 @@ __global__ __launch_bounds__(TPB) void top_row_kernel(TopArgs a) {
 // Joins the chunks of a row.
 template <class T, int TPB>
 __global__ __launch_bounds__(TPB) void top_join_kernel(TopArgs a) {
-    __shared__ TopShared<TPB> sh;
+    __shared__ TopShared<TPB, 0> sh;
     const int r = blockIdx.x, tid = threadIdx.x;
     const EntrySource src{a.keys + (int64_t)r * a.splits * a.K, a.splits * a.K};
     uint32_t top[4] = {0, 0, 0, 0};
     for (int p = tid; p < src.n; p += 4 * TPB) {
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-            if (p + u * TPB < src.n) top[u] = max(top[u], (uint32_t)(src.list[p + u * TPB] >> 32));
+            if (p + u * TPB < src.n) top[u] = max(top[u], pair_value(src.list[p + u * TPB]));
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) sh.keys[u * TPB + tid] = top[u];
@@ -369,8 +526,7 @@ __global__ __launch_bounds__(TPB) void top_join_kernel(TopArgs a) {
         const double total = join_lse(a.parts + (int64_t)r * a.splits, a.splits);
         if (tid == TPB - 1) a.lse[r] = (float)total;
     }
-    const int n = find_candidates<TPB>(src, sh, a.K, nullptr);
-    __syncthreads();
+    const int n = find_candidates<TPB>(src, sh, a.K, [&](uint32_t bound) { scan_all<TPB>(src, sh, bound, true); });
     rank_candidates<TPB>(sh, n, a.K, [&](int place, uint64_t x) { put_out<T>(a, (int64_t)r * a.K + place, x); });
 }
 
@@ -399,16 +555,21 @@ __global__ __launch_bounds__(256) void top_small_kernel(TopArgs a, int rows) {
 // A wave per row where a wave's 256 groups suffice for K and a row is short: no barrier is waited at.
 bool one_wave(const gscan_rows &rows, int K) { return K <= 64 && rows.V <= 2048; }
 
-template <class T, int TPB>
+template <class T, int TPB, int PIECES>
 int launch_rows(const TopArgs &a, int64_t grid, bool lse, hipStream_t stream) {
     const dim3 blocks((unsigned)grid);
-    const bool held = a.chunk <= 4 * TPB * T::vec;
-    if (lse && held) hipLaunchKernelGGL((top_row_kernel<T, TPB, true, true>), blocks, dim3(TPB), 0, stream, a);
-    else if (lse) hipLaunchKernelGGL((top_row_kernel<T, TPB, true, false>), blocks, dim3(TPB), 0, stream, a);
-    else if (held) hipLaunchKernelGGL((top_row_kernel<T, TPB, false, true>), blocks, dim3(TPB), 0, stream, a);
-    else hipLaunchKernelGGL((top_row_kernel<T, TPB, false, false>), blocks, dim3(TPB), 0, stream, a);
+    if (lse) hipLaunchKernelGGL((top_row_kernel<T, TPB, true, PIECES>), blocks, dim3(TPB), 0, stream, a);
+    else hipLaunchKernelGGL((top_row_kernel<T, TPB, false, PIECES>), blocks, dim3(TPB), 0, stream, a);
     GSCAN_LAUNCHED("top_row_kernel");
     return 0;
+}
+// the pieces' maxima: all of them in 8 KB (rows of 32768 16-bit words), else in 16 KB, with groups of pieces from there on
+template <class T, int TPB>
+int launch_rows(const TopArgs &a, int64_t grid, bool lse, hipStream_t stream) {
+    const int pieces = cdiv(a.chunk, T::vec);
+    if (pieces <= 4 * TPB) return launch_rows<T, TPB, 0>(a, grid, lse, stream);
+    if (pieces <= 16 * TPB) return launch_rows<T, TPB, 16 * TPB>(a, grid, lse, stream);
+    return launch_rows<T, TPB, 32 * TPB>(a, grid, lse, stream);
 }
 template <class T>
 int launch_rows(const TopArgs &a, int64_t grid, bool lse, bool wave, hipStream_t stream) {
