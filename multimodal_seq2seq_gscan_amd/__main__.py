@@ -1,7 +1,8 @@
 """Command line of the reference (`python -m seq2seq --mode=train ...`, seq2seq/__main__.py:21-167).
 
-Flag names, defaults and the paired on/off switches are the reference's; two flags are additive:
-`--synthetic_data` trains on seeded synthetic batches of the data set's shape (no dataset file ships
+Flag names, defaults and the paired on/off switches are the reference's; what is additive (the comments in the table
+below): `--beam_size` / `--length_penalty` decode by beam search, `--teacher_from_file` / `--distill_*` train against a
+teacher, `--synthetic_data` trains on seeded synthetic batches of the data set's shape (no dataset file ships
 with the reference checkout, .MISSING_LARGE_BLOBS) and `--synthetic_batches` bounds that run.
 Data-parallel runs are launched with `python -m torch.distributed.run --nproc-per-node N -m seq2seq ...`;
 each rank then trains on its shard of every global batch (train.py in this package).
@@ -35,6 +36,10 @@ _VALUE_FLAGS = [
     ("synthetic_batches", int, 1000),
     # additive: order every window of this many batches by target length after the shuffle (0 = the reference's order)
     ("length_bucket_batches", int, 0),
+    # additive: beam search in the place of greedy decoding (evaluation and --mode=test)
+    ("beam_size", int, 1), ("length_penalty", float, 0.0),
+    # additive: train against a teacher's checkpoint as well
+    ("teacher_from_file", str, ""), ("distill_weight", float, 0.5), ("distill_temperature", float, 2.0), ("distill_top_k", int, 4),
 ]
 # paired switches: (destination, flag that sets True, flag that sets False, default)
 _SWITCHES = [
@@ -121,7 +126,8 @@ def _test_on_dataset(flags) -> None:
         logger.info("Loaded checkpoint '{}' (iter {})".format(flags["resume_from_file"], model.trained_iterations))
         output_file_path = os.path.join(flags["output_directory"], "_".join([split, flags["output_file_name"]]))
         predict_and_save(test_set, model, output_file_path, flags["max_decoding_steps"],
-                         max_testing_examples=flags["max_testing_examples"])
+                         max_testing_examples=flags["max_testing_examples"], beam_size=flags["beam_size"],
+                         length_penalty=flags["length_penalty"])
         logger.info("Saved predictions to {}".format(output_file_path))
 
 
@@ -159,12 +165,17 @@ def main(flags):
         if flags["resume_from_file"]:
             assert os.path.isfile(flags["resume_from_file"]), "No checkpoint found at {}".format(flags["resume_from_file"])
             optimizer_state = model.load_model(flags["resume_from_file"])      # train.py:81-82
+        teacher = {}
+        if flags["teacher_from_file"]:
+            assert os.path.isfile(flags["teacher_from_file"]), "No checkpoint found at {}".format(flags["teacher_from_file"])
+            teacher = dict(teacher=Model.from_checkpoint(flags["teacher_from_file"], **cfg), distill_weight=flags["distill_weight"],
+                           distill_temperature=flags["distill_temperature"], distill_top_k=flags["distill_top_k"])
         step = train(_synthetic_batches(flags, rank, world), model, flags["max_training_iterations"],
                      print_every=flags["print_every"], weight_target_loss=flags["weight_target_loss"], rank=rank,
                      optimizer_state_dict=optimizer_state,
                      learning_rate=flags["learning_rate"], adam_beta_1=flags["adam_beta_1"],
                      adam_beta_2=flags["adam_beta_2"], lr_decay=flags["lr_decay"],
-                     lr_decay_steps=flags["lr_decay_steps"])
+                     lr_decay_steps=flags["lr_decay_steps"], **teacher)
         if rank == 0:
             model.save_checkpoint("checkpoint.pth.tar", is_best=False, optimizer_state_dict=step.optimizer.state_dict())
         logger.info("Finished training.")
@@ -203,7 +214,8 @@ def main(flags):
             output = []
             for (inp, derivation, situation, out_seq, tgt, aw_c, aw_s, pos_acc) in predict(
                     iterator(), model=model, max_decoding_steps=flags["max_decoding_steps"],
-                    pad_idx=cfg["target_pad_idx"], sos_idx=1, eos_idx=cfg["target_eos_idx"]):
+                    pad_idx=cfg["target_pad_idx"], sos_idx=1, eos_idx=cfg["target_eos_idx"], beam_size=flags["beam_size"],
+                    length_penalty=flags["length_penalty"]):
                 accuracy = sequence_accuracy(out_seq, tgt[0].tolist()[1:-1])
                 output.append({"input": inp[0].tolist()[1:-1], "prediction": out_seq, "derivation": derivation,
                                "target": tgt[0].tolist()[1:-1], "situation": situation,

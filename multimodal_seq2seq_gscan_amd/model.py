@@ -25,6 +25,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
+from .logits import distillation_loss
 
 logger = logging.getLogger(__name__)
 
@@ -592,6 +593,14 @@ class Model(nn.Module):
     def get_loss(self, target_scores: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
         return _SequenceNLL.apply(target_scores, targets.contiguous(), self.target_pad_idx)
 
+    def get_distillation_loss(self, target_scores: torch.Tensor, targets: torch.Tensor, teacher_indices: torch.Tensor,
+                              teacher_scores: torch.Tensor, temperature: float = 2.0, weight: float = 0.5) -> torch.Tensor:
+        """`get_loss` against a teacher as well (not in the reference): the mean over the live target positions, the same
+        ones, of  (1 - weight) * NLL + weight * temperature^2 * KL(teacher's top words || student), with the teacher's top
+        words as `logits.top_logits` of its own log-probabilities gives them, [B,T,K] indices and values."""
+        return distillation_loss(target_scores, teacher_indices, teacher_scores, targets, temperature=temperature,
+                                 soft_weight=weight, hard_weight=1.0 - weight, ignore_index=self.target_pad_idx, shift_labels=True)
+
     def get_auxiliary_loss(self, auxiliary_scores_target: torch.Tensor, target_target_positions: torch.Tensor):
         return _PositionNLL.apply(auxiliary_scores_target, target_target_positions.view(-1).contiguous())
 
@@ -799,6 +808,29 @@ class Model(nn.Module):
                           ("best_exact_match", "best_exact_match"), ("best_accuracy", "best_accuracy")):
             setattr(self, attr, checkpoint[key])
         return checkpoint["optimizer_state_dict"]
+
+    @classmethod
+    def from_checkpoint(cls, path_to_checkpoint: str, device="cuda", **cfg) -> "Model":
+        """A model of the sizes that a checkpoint was written with (a teacher need not have its student's): hidden sizes,
+        embedding width, layers, kernel size and vocabularies are read from the shapes of its parameters, the rest (padding
+        indices, output directory, ...) is `cfg`."""
+        state = torch.load(path_to_checkpoint, map_location="cpu")["state_dict"]
+        rows = lambda name: state[name].shape[0]                  # noqa: E731
+        layers = 1
+        while f"encoder.lstm.weight_ih_l{layers}" in state:
+            layers += 1
+        conv_1, conv_3 = state["situation_encoder.conv_1.weight"], state["situation_encoder.conv_3.weight"]
+        cfg.update(input_vocabulary_size=rows("encoder.embedding.weight"),
+                   embedding_dimension=state["encoder.embedding.weight"].shape[1],
+                   encoder_hidden_size=state["encoder.lstm.weight_hh_l0"].shape[1], num_encoder_layers=layers,
+                   encoder_bidirectional="encoder.lstm.weight_hh_l0_reverse" in state,
+                   target_vocabulary_size=rows("attention_decoder.embedding.weight"),
+                   decoder_hidden_size=state["attention_decoder.lstm.weight_hh_l0"].shape[1],
+                   num_cnn_channels=conv_1.shape[1], cnn_hidden_num_channels=conv_1.shape[0], cnn_kernel_size=conv_3.shape[-1],
+                   conditional_attention="attention_decoder.queries_to_keys.weight" in state)
+        model = cls(**cfg).to(device)
+        model.load_model(path_to_checkpoint)
+        return model
 
     def save_checkpoint(self, file_name: str, is_best: bool, optimizer_state_dict: dict) -> str:
         path = os.path.join(self.output_directory, file_name)

@@ -14,7 +14,9 @@ from typing import Iterator, List, Tuple
 
 import torch
 
+from . import _lib
 from ._lib import GscanError
+from .logits import beam_reorder, beam_select
 
 logger = logging.getLogger(__name__)
 
@@ -102,8 +104,73 @@ def greedy_decode_stepwise(model, commands: torch.Tensor, cmd_lengths, world: to
     return rows
 
 
+def beam_decode(model, commands: torch.Tensor, cmd_lengths, world: torch.Tensor, sos_idx: int, eos_idx: int,
+                max_decoding_steps: int, beam_size: int, pad_idx: int = 0, length_penalty: float = 0.0) -> dict:
+    """Beam search (not in the reference) in the place of `greedy_decode`, with its limits: `beam_size` continuations of
+    every row are kept per step (`logits.beam_select`), the decoder's states follow their beams (`logits.beam_reorder`), and a
+    row's answer is the beam of the largest  log-probability / length ** length_penalty  after max_decoding_steps + 1 steps or
+    when all beams of all rows have ended.  Returns greedy_decode's dictionary, the attention rows being those along the
+    answer, and `scores`, the answers' log-probabilities.  A beam of 1 decodes greedily.
+
+    The rows' commands and worlds are encoded once per beam, so that beams are rows to the decoder's step kernel; words,
+    parents and attention rows stay on the device until the search has ended, and the host looks at it every eighth step."""
+    B, W, device = commands.shape[0], int(beam_size), commands.device
+    if not 1 <= W <= _lib.MAX_BEAMS:
+        raise ValueError(f"beam_size must be 1 to {_lib.MAX_BEAMS}, got {beam_size}")
+    lengths = [int(v) for v in (cmd_lengths.tolist() if isinstance(cmd_lengths, torch.Tensor) else cmd_lengths)]
+    per_beam = [n for n in lengths for _ in range(W)]
+    encoded = model.encode_input(commands_input=commands.repeat_interleave(W, 0), commands_lengths=per_beam,
+                                 situations_input=world.repeat_interleave(W, 0))
+    keys_vis = model.visual_attention.key_layer(encoded["encoded_situations"])
+    keys_txt = model.textual_attention.key_layer(encoded["encoded_commands"]["encoder_outputs"])
+    hidden = model.attention_decoder.initialize_hidden(model.tanh(model.enc_hidden_to_dec_hidden(encoded["hidden_states"])))
+    per_beam = torch.tensor(per_beam, dtype=torch.int32)
+    words = torch.full((B, W), sos_idx, dtype=torch.long, device=device)
+    scores = torch.full((B, W), float("-inf"), device=device)
+    scores[:, 0] = 0.0
+    finished = torch.zeros(B, W, dtype=torch.bool, device=device)
+    trace = []
+    for it in range(int(max_decoding_steps) + 1):
+        logits, (h, c), _, alpha_text, alpha_vis = model.decode_input(
+            target_token=words.view(-1), hidden=hidden, encoder_outputs=keys_txt, input_lengths=per_beam, encoded_situations=keys_vis)
+        scores, parents, words, finished = beam_select(logits.view(B, W, -1), scores, finished, eos_idx=eos_idx, pad_idx=pad_idx)
+        hidden = tuple(beam_reorder(parents, [h, c], dim=1))
+        trace.append((parents, words, alpha_text, alpha_vis))
+        if it % 8 == 7 and bool(finished.all()):
+            break
+    S = len(trace)
+    parents = torch.stack([t[0] for t in trace]).cpu().tolist()
+    chosen = torch.stack([t[1] for t in trace]).cpu().tolist()
+    at = torch.stack([t[2] for t in trace]).view(S, B, W, -1).cpu()
+    av = torch.stack([t[3] for t in trace]).view(S, B, W, -1).cpu()
+    final = scores.cpu().tolist()
+    rows = {"tokens": [], "alpha_text": [], "alpha_vis": [], "scores": []}
+    att_sum = torch.zeros(B, av.shape[-1])
+    for r in range(B):
+        best = None
+        for w in range(W):
+            path, slot = [], w                      # (beam that the step ran on, word), last step first
+            for s in range(S - 1, -1, -1):
+                path.append((parents[s][r][slot], chosen[s][r][slot]))
+                slot = parents[s][r][slot]
+            path.reverse()
+            tokens = [v for _, v in path]
+            n = tokens.index(eos_idx) + 1 if eos_idx in tokens else S
+            value = final[r][w] / n ** length_penalty
+            if best is None or value > best[0]:
+                best = (value, path[:n], final[r][w])
+        _, path, score = best
+        rows["tokens"].append([v for _, v in path])
+        rows["alpha_text"].append([at[s, r, b, :lengths[r]].tolist() for s, (b, _) in enumerate(path)])
+        rows["alpha_vis"].append([av[s, r, b].tolist() for s, (b, _) in enumerate(path)])
+        rows["scores"].append(score)
+        att_sum[r] = sum(av[s, r, b] for s, (b, _) in enumerate(path))
+    rows["att_sum"] = att_sum.to(device)
+    return rows
+
+
 def predict(data_iterator: Iterator, model, max_decoding_steps: int, pad_idx: int, sos_idx: int, eos_idx: int,
-            max_examples_to_evaluate=None) -> Iterator[Tuple]:
+            max_examples_to_evaluate=None, beam_size: int = 1, length_penalty: float = 0.0) -> Iterator[Tuple]:
     """predict.py:57-128.  `data_iterator` yields the reference's 9-tuples (gSCAN_dataset.py:229-231) with any batch
     size; one 8-tuple is yielded per example:
     (input_sequence [1,L], derivation_spec, situation_spec, output_sequence, target_sequence [1,T],
@@ -115,7 +182,11 @@ def predict(data_iterator: Iterator, model, max_decoding_steps: int, pad_idx: in
         for (input_sequence, input_lengths, derivation_spec, situation, situation_spec, target_sequence,
              target_lengths, agent_positions, target_positions) in data_iterator:
             B = input_sequence.shape[0]
-            rows = greedy_decode(model, input_sequence, input_lengths, situation, sos_idx, eos_idx, max_decoding_steps)
+            if beam_size > 1:
+                rows = beam_decode(model, input_sequence, input_lengths, situation, sos_idx, eos_idx, max_decoding_steps,
+                                   beam_size, pad_idx, length_penalty)
+            else:
+                rows = greedy_decode(model, input_sequence, input_lengths, situation, sos_idx, eos_idx, max_decoding_steps)
             aux_scores = model.auxiliary_task_forward(rows["att_sum"]) if model.auxiliary_task else None
             for r in range(B):
                 count += 1
@@ -136,13 +207,14 @@ def predict(data_iterator: Iterator, model, max_decoding_steps: int, pad_idx: in
 
 
 def evaluate_sums(data_iterator: Iterator, model, max_decoding_steps: int, pad_idx: int, sos_idx: int, eos_idx: int,
-                  max_examples_to_evaluate=None) -> Tuple[float, float, float, float]:
+                  max_examples_to_evaluate=None, beam_size: int = 1, length_penalty: float = 0.0) -> Tuple[float, float, float, float]:
     """The sums behind evaluate(): (sum of token accuracies %, exact matches, sum of target-position accuracies %,
     examples) — additive over shards of a split, which is how data-parallel ranks share an evaluation."""
     acc_sum, target_sum, exact, n = 0.0, 0.0, 0, 0
     for _, _, _, output_sequence, target_sequence, _, _, aux_acc_target in predict(
             data_iterator=data_iterator, model=model, max_decoding_steps=max_decoding_steps, pad_idx=pad_idx,
-            sos_idx=sos_idx, eos_idx=eos_idx, max_examples_to_evaluate=max_examples_to_evaluate):
+            sos_idx=sos_idx, eos_idx=eos_idx, max_examples_to_evaluate=max_examples_to_evaluate, beam_size=beam_size,
+            length_penalty=length_penalty):
         accuracy = sequence_accuracy(output_sequence, target_sequence[0].tolist()[1:-1])
         exact += int(accuracy == 100)
         acc_sum += accuracy
@@ -152,15 +224,15 @@ def evaluate_sums(data_iterator: Iterator, model, max_decoding_steps: int, pad_i
 
 
 def evaluate(data_iterator: Iterator, model, max_decoding_steps: int, pad_idx: int, sos_idx: int, eos_idx: int,
-             max_examples_to_evaluate=None) -> Tuple[float, float, float]:
+             max_examples_to_evaluate=None, beam_size: int = 1, length_penalty: float = 0.0) -> Tuple[float, float, float]:
     """evaluate.py:10-24: (mean token accuracy %, exact match %, mean target-position accuracy %)."""
     acc_sum, exact, target_sum, n = evaluate_sums(data_iterator, model, max_decoding_steps, pad_idx, sos_idx, eos_idx,
-                                                  max_examples_to_evaluate)
+                                                  max_examples_to_evaluate, beam_size, length_penalty)
     return acc_sum / n, (exact / n) * 100, target_sum / n
 
 
 def predict_and_save(dataset, model, output_file_path: str, max_decoding_steps: int, max_testing_examples=None,
-                     batch_size: int = 256, **kwargs) -> str:
+                     batch_size: int = 256, beam_size: int = 1, length_penalty: float = 0.0, **kwargs) -> str:
     """seq2seq/predict.py:16-54: decode every example of `dataset` and write the reference's record schema
     (input, prediction, derivation, target, situation, both attention traces, accuracy, exact_match,
     position_accuracy) as JSON.  Batched (the reference iterates with batch_size=1)."""
@@ -169,7 +241,7 @@ def predict_and_save(dataset, model, output_file_path: str, max_decoding_steps: 
             dataset.get_data_iterator(batch_size=batch_size, world_dtype=torch.uint8), model=model,
             max_decoding_steps=max_decoding_steps,
             pad_idx=vocab.pad_idx, sos_idx=vocab.sos_idx, eos_idx=vocab.eos_idx,
-            max_examples_to_evaluate=max_testing_examples):
+            max_examples_to_evaluate=max_testing_examples, beam_size=beam_size, length_penalty=length_penalty):
         accuracy = sequence_accuracy(out_seq, tgt[0].tolist()[1:-1])
         output.append({"input": dataset.array_to_sentence(inp[0].tolist(), "input")[1:-1],
                        "prediction": dataset.array_to_sentence(out_seq, "target"), "derivation": derivation,

@@ -26,6 +26,7 @@ import torch
 import torch.distributed as dist
 
 from . import _lib
+from .logits import _distillation, _launch_distillation, top_logits
 from .model import Model, _as_int32_lengths
 
 logger = logging.getLogger(__name__)
@@ -414,12 +415,30 @@ class TrainStep:
                  weight_target_loss: float = 0.3, process_group=None,
                  fused_loss: Optional[bool] = None, single_exchange: Optional[bool] = None,
                  always_collective: bool = False, on_gradients=None,
-                 native_allreduce: Optional[bool] = None, dp_buckets: Optional[int] = None, **ignored):
+                 native_allreduce: Optional[bool] = None, dp_buckets: Optional[int] = None, teacher: Optional[Model] = None,
+                 distill_weight: float = 0.5, distill_temperature: float = 2.0, distill_top_k: int = 4, **ignored):
         if ignored.pop("graph", None):
             # hipGraph replay left the product path in round 4 (slower than eager launches on this stack)
             logger.warning("TrainStep(graph=True): graph replay is no longer available, the step launches eagerly")
         if ignored:                                          # the reference's callers pass their whole flag dict (model.py:26-32)
             logger.debug("TrainStep: ignoring arguments %s", sorted(ignored))
+        # A teacher (not in the reference): the sequence loss becomes Model.get_distillation_loss against the teacher's top
+        # `distill_top_k` words of every position, teacher-forced on the same batch without dropout.
+        self.teacher = teacher
+        if teacher is not None:
+            if teacher is model:
+                raise ValueError("a model cannot be its own teacher: one step is in flight per model")
+            if teacher._hyper["V"] != model._hyper["V"] or teacher._hyper["Vi"] != model._hyper["Vi"] or teacher._hyper["C"] != model._hyper["C"]:
+                raise ValueError("teacher and student must share their vocabularies and the world's channels")
+            if not 0.0 <= float(distill_weight) <= 1.0:
+                raise ValueError(f"distill_weight must be 0 to 1, got {distill_weight}")
+            if int(distill_top_k) < 1:
+                raise ValueError(f"distill_top_k must be at least 1, got {distill_top_k}")
+            if fused_loss or single_exchange:
+                raise ValueError("a step with a teacher exchanges its statistics before the backward pass")
+            fused_loss = single_exchange = False
+            teacher.eval()
+        self.distill = (float(distill_weight), float(distill_temperature), min(int(distill_top_k), model._hyper["V"], _lib.MAX_TOP))
         self.model = model
         self.optimizer = FlatAdam(model, learning_rate, adam_beta_1, adam_beta_2, lr_decay, lr_decay_steps)
         self.weight_target_loss = float(weight_target_loss)
@@ -484,6 +503,8 @@ class TrainStep:
         logp, aux, call = model._launch_forward(commands, batch["cmd_lengths"], world, targets, masks, pos)
         if self.fused_loss or self.single_exchange:
             return {"logp": logp, "aux": aux, "call": call}
+        if self.teacher is not None:
+            return dict(self._distill(batch, logp, aux), logp=logp, aux=aux, call=call)
         dlogp = torch.empty_like(logp)
         daux = torch.empty_like(aux) if model.auxiliary_task else None
         pos = batch["target_positions"].view(-1).contiguous() if model.auxiliary_task else None
@@ -493,6 +514,29 @@ class TrainStep:
                                          model.target_pad_idx, self.stats.data_ptr(), dlogp.data_ptr(),
                                          _lib.ptr(daux), stream), "gscan_step_losses")
         return {"logp": logp, "aux": aux, "call": call, "dlogp": dlogp, "daux": daux, "pos": pos}
+
+    def _distill(self, batch, logp: torch.Tensor, aux: Optional[torch.Tensor]) -> dict:
+        """What gscan_step_losses gives a step without a teacher: statistics [sum of the sequence losses, tokens, sum aux NLL,
+        rows] and the gradients of the two sums."""
+        model, teacher = self.model, self.teacher
+        weight, temperature, k = self.distill
+        with torch.no_grad():
+            scores, _, _ = teacher._launch_forward(batch["commands"], batch["cmd_lengths"], batch["world"], batch["targets"],
+                                                   (None, None, None))
+            values, indices = top_logits(scores, k)
+        device, logits, rows, terms, _kept = _distillation(logp, indices, values, batch["targets"], temperature, weight, 1.0 - weight,
+                                                           model.target_pad_idx, True, "sum")
+        dlogp = torch.empty_like(logits)
+        _launch_distillation(device, logits, rows, terms, None, dlogp, stats=self.stats)
+        daux = None
+        if model.auxiliary_task:
+            daux = torch.empty_like(aux)
+            pos = batch["target_positions"].view(-1).contiguous()
+            _lib.check(_lib.load().gscan_position_nll(aux.data_ptr(), pos.data_ptr(), aux.shape[0], aux.shape[1],
+                                                      self.stats.data_ptr() + 8, daux.data_ptr(),
+                                                      torch.cuda.current_stream().cuda_stream), "gscan_position_nll")
+            self.stats[3:].fill_(float(aux.shape[0]))
+        return {"dlogp": dlogp, "daux": daux}
 
     def _section_backward(self, fw: dict) -> None:
         lib = _lib.load()
@@ -600,7 +644,8 @@ def train_on_dataset(data_path: str, data_directory: str, generate_vocabularies:
                      print_every: int, evaluate_every: int, max_decoding_steps: int, output_directory: str,
                      resume_from_file: str = "", k: int = 0, max_training_examples=None, max_testing_examples=None,
                      weight_target_loss: float = 0.3, seed: int = 42, rank: int = 0, world_size: int = 1,
-                     evaluation_batch_size: int = 256, length_bucket_batches: int = 0, **flags) -> Model:
+                     evaluation_batch_size: int = 256, length_bucket_batches: int = 0, teacher_from_file: str = "",
+                     beam_size: int = 1, length_penalty: float = 0.0, **flags) -> Model:
     """seq2seq/train.py:17-154 on a gSCAN dataset file: the reference's loop — shuffle, iterate batches, step,
     log every `print_every`, greedy-decode the dev split every `evaluate_every` and checkpoint on a new best exact
     match — with the HIP step, the packed batcher (dataset.py) and batched evaluation.  Under torch.distributed
@@ -646,6 +691,11 @@ def train_on_dataset(data_path: str, data_directory: str, generate_vocabularies:
     model = Model(**cfg).cuda()
     optim = {key: flags[key] for key in ("learning_rate", "adam_beta_1", "adam_beta_2", "lr_decay", "lr_decay_steps")
              if key in flags}
+    if teacher_from_file:
+        assert os.path.isfile(teacher_from_file), "No checkpoint found at {}".format(teacher_from_file)
+        optim.update(teacher=Model.from_checkpoint(teacher_from_file, **cfg),
+                     **{key: flags[key] for key in ("distill_weight", "distill_temperature", "distill_top_k") if key in flags})
+        logger.info("Teacher: '{}'".format(teacher_from_file))
     step = TrainStep(model, weight_target_loss=weight_target_loss, **optim)
     best_exact_match = 0
     if resume_from_file:
@@ -687,7 +737,8 @@ def train_on_dataset(data_path: str, data_directory: str, generate_vocabularies:
                     dev_set.get_data_iterator(batch_size=evaluation_batch_size, shard=(rank, world_size),
                                               world_dtype=torch.uint8), model=model,
                     max_decoding_steps=max_decoding_steps, pad_idx=vocab.pad_idx, sos_idx=vocab.sos_idx,
-                    eos_idx=vocab.eos_idx, max_examples_to_evaluate=limit), dtype=torch.float64)
+                    eos_idx=vocab.eos_idx, max_examples_to_evaluate=limit, beam_size=beam_size,
+                    length_penalty=length_penalty), dtype=torch.float64)
                 if world_size > 1:
                     sums = step.exchange.all_reduce(sums.cuda()).cpu()
                 n = max(float(sums[3]), 1.0)
