@@ -81,6 +81,16 @@ def _init_distributed():
     return rank, world
 
 
+def _end_distributed() -> None:
+    """Ends the process group that this run created.  Without it a transport thread of gloo can still be giving back
+    the tensors of the last collective when the interpreter shuts down: it then waits for an interpreter lock that
+    nobody hands out any more, its thread is cancelled inside a destructor, and the process aborts after its work
+    was done (12 of 80 two-rank CPU processes whose lock changes hands seldom; none of 80 with the group ended)."""
+    import torch.distributed as dist
+    if dist.is_available() and dist.is_initialized():
+        dist.destroy_process_group()
+
+
 def _synthetic_batches(flags, rank: int, world: int):
     from .synthetic import Shape, make_batch
     from .train import shard_batch
@@ -151,12 +161,16 @@ def main(flags):
         from .train import train
         if not torch.cuda.is_available():
             raise RuntimeError("training runs on the HIP device only (no CPU fallback in this package)")
+        import torch.distributed as dist
+        owned = not (dist.is_available() and dist.is_initialized())       # a caller's own process group stays as it is
         rank, world = _init_distributed()
         torch.manual_seed(flags["seed"])                      # train.py:27 (identical init on every rank)
         if not flags["synthetic_data"]:
             from .train import train_on_dataset
             train_on_dataset(data_path=os.path.join(flags["data_directory"], "dataset.txt"), rank=rank,
                              world_size=world, **flags)
+            if owned:
+                _end_distributed()
             return
         cfg = model_kwargs("compositional")
         cfg.update({k: flags[k] for k in cfg if k in flags})
@@ -178,7 +192,10 @@ def main(flags):
                      lr_decay_steps=flags["lr_decay_steps"], **teacher)
         if rank == 0:
             model.save_checkpoint("checkpoint.pth.tar", is_best=False, optimizer_state_dict=step.optimizer.state_dict())
+        step.close()                                          # the library's RCCL communicator, before the process group goes
         logger.info("Finished training.")
+        if owned:
+            _end_distributed()
     elif flags["mode"] == "test":
         # seq2seq/__main__.py:124-163 + predict.py:17-54: greedy-decode every example of each split and write
         # <split>_<output_file_name> with the reference's record schema.  Synthetic data has no vocabulary, so the
