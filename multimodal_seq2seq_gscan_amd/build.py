@@ -34,14 +34,15 @@ def units():
             out.append((src, obj, EXTRA_FLAGS.get(src, []) + ([f"-DGSCAN_DEC_PART={k}"] if n > 1 else [])))
     return out
 
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
+# No packed fp32 instructions: some forms that the compiler makes of ordinary float code have given wrong results now and
+# then on this hardware.  The same sums of the same roundings take two instructions in place of one: the training step of
+# the compositional configuration takes 0.434 in place of 0.424 ms.  (The host pass warns that it does not know the feature.)
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", *NO_PACKED_FP32,
          f"-I{INCLUDE}", f"-I{CSRC}"]
 # per-source extras: the grouped GEMM's problem lookup reads its header from preloaded kernel-argument SGPRs
 EXTRA_FLAGS = {"gemm.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=12"],
-               "gemm_mt.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=12"],
-               # no packed fp32 instructions in the operators over rows of logits
-               **{src: ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-                  for src in ("top_logits.hip", "distill.hip", "beam.hip")}}
+               "gemm_mt.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=12"]}
 
 
 def _hipcc() -> str:

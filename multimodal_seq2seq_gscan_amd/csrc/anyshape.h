@@ -18,8 +18,8 @@ __device__ __forceinline__ int any_tid() {
     return t;
 }
 
-// acc += w . v as two packed FMAs on register pairs that come out of ONE 16-byte load each ((x, y) and (z, w)).  Written as four
-// scalar FMAs per row, the compiler packed ACROSS rows instead ({w[u].x, w[u+1].x} ...), shuffled every loaded float4 into
+// acc += w . v as two pairs of FMAs on registers that come out of ONE 16-byte load each ((x, y) and (z, w)).  Written as four
+// scalar FMAs per row, and with packed fp32 allowed, the compiler packed ACROSS rows instead ({w[u].x, w[u+1].x} ...), shuffled every loaded float4 into
 // that layout with v_mov right behind the loads, and so waited for the loads two at a time (the ISA of round 4's kernels):
 // a thread never had more than 32 bytes in flight, whatever the source said.
 using any_f32x2 = __attribute__((ext_vector_type(2))) float;

@@ -78,8 +78,8 @@ __device__ __forceinline__ int opaque(int x) {
 // (row_half_mirror); both lanes must be active and both end up with the sum
 __device__ __forceinline__ float pair_sum(float v) { return v + dpp_move<0x141, 0xf>(v); }
 
-// Dot products of register-resident half rows with an LDS vector (K0 % 4 == 0), as packed FMAs
-// (v_pk_fma_f32).  The vector is read in chunks of four float4; the next chunk's reads are issued before the
+// Dot products of register-resident half rows with an LDS vector (K0 % 4 == 0), in pairs of FMAs
+// (two accumulators of two lanes; no packed instructions, build.py).  The vector is read in chunks of four float4; the next chunk's reads are issued before the
 // current chunk's FMAs, so the LDS latency is paid about once per dot instead of once per read.
 constexpr int kWaitVmcnt0 = 0x0F70;   // s_waitcnt vmcnt(0) only (gfx9 encoding: expcnt 7, lgkmcnt 15 = no wait)
 #ifndef GSCAN_DEC_DOT_CHUNK
@@ -438,8 +438,8 @@ __device__ __forceinline__ float quad_bcast(float v) { return dpp_move<I * 0x55,
 #define GSCAN_DEC_QCS_U 3
 #endif
 // The same sum when n is a whole number of rounds (n % (4 U) == 0: the 36 cells of a 6 x 6 grid are three rounds of
-// twelve): no clamped indices, no masked weights, addresses by addition — per memory one LDS read, one ds_bpermute and two
-// packed FMAs instead of those plus a min, a 24-bit multiply, two shifts, a compare and a select (round 6: the column-sum
+// twelve): no clamped indices, no masked weights, addresses by addition — per memory one LDS read, one ds_bpermute and
+// four FMAs instead of those plus a min, a 24-bit multiply, two shifts, a compare and a select (round 6: the column-sum
 // phases are bound by instruction issue, two waves per SIMD).
 #ifndef GSCAN_DEC_QCS_EXACT
 #define GSCAN_DEC_QCS_EXACT 1

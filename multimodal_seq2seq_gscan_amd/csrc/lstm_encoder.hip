@@ -23,8 +23,8 @@ namespace gscan {
 template <int HE, int R>
 __device__ __forceinline__ void dots_lds(const float (&w)[R][HE], const float *v, float (&out)[R]) {
     static_assert(HE % 4 == 0, "hidden size must be a multiple of 4");
-    // packed FMAs (v_pk_fma_f32: two lanes of a register pair per instruction): with two workgroups per CU the
-    // recurrence's step was bound by the issue of these FMAs (2 waves x 200 scalar FMAs x 4 cycles of the ~2 000 per step)
+    // two accumulators of two lanes: with two workgroups per CU the recurrence's step is bound by the issue of these
+    // FMAs (2 waves x 200 scalar FMAs x 4 cycles of the ~2 000 per step; packed fp32 would halve them, build.py)
     using f32x2 = __attribute__((ext_vector_type(2))) float;
     f32x2 a01[R], a23[R];
 #pragma unroll
