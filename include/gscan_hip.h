@@ -330,7 +330,7 @@ int gscan_comm_set_early_allreduce(void *comm, float *buf, size_t n);
 #define GSCAN_MAX_BEAMS 64
 
 /* Rows of V adjacent words: row (o, i), 0 <= o < outer, 0 <= i < inner, begins at element o * stride_outer + i * stride_inner
- * of `data`.  A row may begin at any element.  1 <= outer * inner <= 2^24, V <= 2^30. */
+ * of `data`.  A row may begin at any element.  1 <= outer * inner < 2^23, V <= 2^30. */
 typedef struct gscan_rows {
     const void *data;
     int32_t type;              /* GSCAN_F32, GSCAN_BF16, GSCAN_F16                  */
@@ -367,9 +367,9 @@ typedef struct gscan_distillation {
 
 /* With p = softmax(teacher / temperature) over a row's entries, q = softmax(z / temperature), s = softmax(z):
  *   loss = mean over the live rows of  hard_weight (-log s[label]) + soft_weight temperature^2 sum_k p_k log(p_k / q[index_k])
- * (a row without entries has no soft term), written to loss[0] (NULL, without stats: the gradient alone).  grad (may be NULL: the loss alone) [outer, inner, V] of the
- * rows' type, contiguous, receives upstream[0] (device scalar, NULL = 1) times d(loss)/d(logits), rounded once; it may not
- * overlap the logits.  stats (may be NULL) [4] = [sum of the rows' losses, live rows, sum of -log s[label], sum of the
+ * (a row without entries has no soft term), written to loss[0] (NULL, without stats: the gradient alone).  grad
+ * (may be NULL: the loss alone) [outer, inner, V] of the rows' type, contiguous, receives upstream[0] (device scalar, NULL = 1)
+ * times d(loss)/d(logits), rounded once; it may not overlap an input.  stats (may be NULL) [4] = [sum of the rows' losses, live rows, sum of -log s[label], sum of the
  * divergences] (of a term whose weight is 0: 0) — what a data-parallel step adds up over its ranks.  Two calls give the same
  * bits. */
 size_t gscan_distillation_workspace_bytes(const gscan_rows *rows);

@@ -182,7 +182,8 @@ BeamPlan beam_plan(const gscan_rows &rows) {
 // ---- reordering ----
 constexpr int kMaxStates = 16;           // per launch: the table travels in the kernel's arguments
 constexpr int kSegment = 4096;           // bytes that a wave copies
-constexpr int64_t kMaxItems = 1 << 28;   // pieces of one state: a launch's blocks stay below 2^31
+constexpr int64_t kMaxItems = 1 << 25;   // segments of one state
+constexpr int64_t kMaxBlocks = (1 << 24) - 1;      // of a launch, which counts its threads in 32 bits
 
 struct CopyState {
     const char *in; char *out;
@@ -305,13 +306,14 @@ int beam_reorder(int B, int W, const int32_t *parents, const gscan_state *states
         GSCAN_CHECK(items <= kMaxItems && items * t.mid <= kMaxItems && items * t.mid * segments <= kMaxItems,
                     "beam_reorder: state %d has too many pieces", k);
     }
-    for (int k0 = 0; k0 < count; k0 += kMaxStates) {
+    for (int k = 0; k < count;) {
         CopyArgs a{};
         a.B = B; a.W = W; a.parents = parents;
         int64_t blocks = 0;
-        for (int k = k0; k < count && k < k0 + kMaxStates; ++k) {
+        for (; k < count && a.count < kMaxStates; ++k) {
             const gscan_state &t = states[k];
-            const int64_t segments = (t.bytes + kSegment - 1) / kSegment;
+            const int64_t segments = (t.bytes + kSegment - 1) / kSegment, own = (t.outer * B * W * t.mid * segments + 3) / 4;
+            if (blocks + own > kMaxBlocks) break;          // a state alone has at most half of them
             CopyState &s = a.s[a.count++];
             s.in = (const char *)t.in; s.out = (char *)t.out;
             s.in_outer = t.in_outer; s.out_outer = t.out_outer; s.in_row = t.in_row; s.out_row = t.out_row;
@@ -321,7 +323,7 @@ int beam_reorder(int B, int W, const int32_t *parents, const gscan_state *states
                                  (uint64_t)t.in_row | (uint64_t)t.out_row | (uint64_t)t.in_mid | (uint64_t)t.out_mid | (uint64_t)t.bytes;
             s.width = all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
             s.first_block = (int)blocks;
-            blocks += (t.outer * B * W * t.mid * segments + 3) / 4;
+            blocks += own;
         }
         hipLaunchKernelGGL(beam_reorder_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
         GSCAN_LAUNCHED("beam_reorder_kernel");

@@ -23,6 +23,9 @@ constexpr int kCountBlocks = 64;
 // less: 22.8 for 27.1 us at 5120 rows of 9 words); longer rows fill the chip with workgroups, and theirs come from a launch
 // before them (4088 rows of 32000 words: 134 for 152 us).
 constexpr int kCountThere = 8192, kCountThereLong = 256;
+// Above so many workgroups their parts are added up by 64 workgroups before the one that finishes (rows of 100 words: 8192 rows
+// 25.6 us without and 28.5 with this launch, 16384: 32.2 and 30.5, 262144: 347 and 275).
+constexpr int kFinishParts = 8192;
 struct DistillArgs {
     Rows rows;
     int count;                         // rows in all
@@ -95,6 +98,22 @@ __global__ __launch_bounds__(256) void distill_count_kernel(DistillArgs a, int *
     if (threadIdx.x == 0) live[blockIdx.x] = s[0] + s[1] + s[2] + s[3];
 }
 
+// Many workgroups' parts, added up to kCountBlocks of them before the last launch, which is one workgroup.
+__global__ __launch_bounds__(256) void distill_add_kernel(const double *part, int n, double *sums) {
+    __shared__ double s[3][4];
+    double v[3] = {0.0, 0.0, 0.0};
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += kCountBlocks * 256) {
+        v[0] += part[3 * (int64_t)i]; v[1] += part[3 * (int64_t)i + 1]; v[2] += part[3 * (int64_t)i + 2];
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        v[k] = wave_reduce(v[k], [](double x, double y) { return x + y; });
+        if ((threadIdx.x & 63) == 0) s[k][threadIdx.x >> 6] = v[k];
+    }
+    __syncthreads();
+    if (threadIdx.x < 3) sums[3 * blockIdx.x + threadIdx.x] = s[threadIdx.x][0] + s[threadIdx.x][1] + s[threadIdx.x][2] + s[threadIdx.x][3];
+}
+
 __global__ __launch_bounds__(1024) void distill_finish_kernel(const double *part, int n, float soft, float hard, int mean, float *loss, float *stats) {
     __shared__ double s[3][16];
     double v[3] = {0.0, 0.0, 0.0};
@@ -156,7 +175,7 @@ template <int TPB>
 __device__ __forceinline__ float gradient_scale(const DistillArgs &a, RowShared<TPB> &sh) {
     if (a.sum) return over_live(a, 0);
     if (a.live) return over_live(a, (int)wave_sum((float)a.live[threadIdx.x & 63]));
-    const float n = wave_sum((float)count_live(a, threadIdx.x, TPB));       // at most 2^24 rows: exact
+    const float n = wave_sum((float)count_live(a, threadIdx.x, TPB));       // fewer than 2^23 rows: exact
     if ((threadIdx.x & 63) == 0) sh.live[threadIdx.x >> 6] = n;
     lds_barrier();
     float all = 0.f;
@@ -514,6 +533,8 @@ __global__ __launch_bounds__(256) void distill_small_kernel(DistillArgs a) {
         }
         share[k] = e;
     }
+    // a row's entries stay within its wave, whose LDS accesses are in order: only the compiler has to keep them so
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     A = lanes(A, plus);
     B = lanes(B, plus);
     const float e0 = in ? __builtin_amdgcn_exp2f((z - zmax) * a.inv_tau * kLog2e) : 0.f;
@@ -610,7 +631,7 @@ int launch_type(const DistillArgs &a, hipStream_t stream) {
 }  // namespace
 
 size_t distillation_workspace(const gscan_rows &rows) {
-    return kCountBlocks * sizeof(int) + (size_t)part_blocks(rows) * 3 * sizeof(double);
+    return kCountBlocks * (sizeof(int) + 3 * sizeof(double)) + (size_t)part_blocks(rows) * 3 * sizeof(double);
 }
 
 int distillation_loss(const gscan_rows &rows, const gscan_distillation &t, const float *upstream, void *grad, float *loss,
@@ -640,7 +661,8 @@ int distillation_loss(const gscan_rows &rows, const gscan_distillation &t, const
     a.soft = t.soft_weight; a.soft_grad = t.soft_weight * t.temperature; a.hard = t.hard_weight;
     a.power = t.temperature == 2.f ? 2 : t.temperature == 3.f ? 3 : t.temperature == 4.f ? 4 : 0;
     a.upstream = upstream; a.grad = (char *)grad;
-    a.part = (double *)(live + kCountBlocks);
+    double *sums = (double *)(live + kCountBlocks);
+    a.part = sums + 3 * kCountBlocks;
     a.sum = t.sum_reduction != 0;
     if (grad && !a.sum && a.count > (rows.V <= 64 ? kCountThere : kCountThereLong)) {       // the gradient of a mean needs the number of live rows first
         a.live = live;
@@ -653,7 +675,15 @@ int distillation_loss(const gscan_rows &rows, const gscan_distillation &t, const
                                 : launch_type<TypeF16>(a, stream));
     if (!loss) return 0;
     const float tau2 = t.temperature * t.temperature;
-    hipLaunchKernelGGL(distill_finish_kernel, dim3(1), dim3(1024), 0, stream, a.part, part_blocks(rows), t.soft_weight * tau2,
+    const double *part = a.part;
+    int parts = part_blocks(rows);
+    if (parts > kFinishParts) {
+        hipLaunchKernelGGL(distill_add_kernel, dim3(kCountBlocks), dim3(256), 0, stream, part, parts, sums);
+        GSCAN_LAUNCHED("distill_add_kernel");
+        part = sums;
+        parts = kCountBlocks;
+    }
+    hipLaunchKernelGGL(distill_finish_kernel, dim3(1), dim3(1024), 0, stream, part, parts, t.soft_weight * tau2,
                        t.hard_weight, t.sum_reduction ? 0 : 1, loss, stats);
     GSCAN_LAUNCHED("distill_finish_kernel");
     return 0;

@@ -603,9 +603,10 @@ int check_rows(const char *who, const gscan_rows *rows) {
     GSCAN_CHECK(rows->data, "%s: logits are NULL", who);
     GSCAN_CHECK(rows->type == GSCAN_F32 || rows->type == GSCAN_BF16 || rows->type == GSCAN_F16, "%s: unknown type %d", who, rows->type);
     GSCAN_CHECK(rows->V >= 1 && rows->V <= (1 << 30), "%s: %d words (1 to 2^30)", who, rows->V);
-    GSCAN_CHECK(rows->outer >= 1 && rows->inner >= 1 && rows->outer <= (1 << 24) && rows->inner <= (1 << 24) &&
-                    rows->outer * rows->inner <= (1 << 24),
-                "%s: %lld x %lld rows (1 to 2^24)", who, (long long)rows->outer, (long long)rows->inner);
+    // a launch counts its threads in 32 bits: 512 a row
+    GSCAN_CHECK(rows->outer >= 1 && rows->inner >= 1 && rows->outer < (1 << 23) && rows->inner < (1 << 23) &&
+                    rows->outer * rows->inner < (1 << 23),
+                "%s: %lld x %lld rows (1 to 2^23 - 1)", who, (long long)rows->outer, (long long)rows->inner);
     GSCAN_CHECK(rows->stride_outer >= 0 && rows->stride_inner >= 0, "%s: negative stride", who);
     const int64_t b = rows->type == GSCAN_F32 ? 4 : 2;
     GSCAN_CHECK(((uintptr_t)rows->data) % b == 0, "%s: logits are not aligned to their type", who);

@@ -65,6 +65,9 @@ def _rows(logits: torch.Tensor) -> Tuple[torch.Tensor, _lib.Rows]:
     if stride[-1] != 1 and V > 1:
         return _rows(logits.contiguous())
     inner, si = (shape[-2], stride[-2]) if n > 1 else (1, 0)
+    if n <= 3:
+        outer, so = (shape[0], stride[0]) if n == 3 else (1, 0)
+        return logits, _lib.Rows(logits.data_ptr(), kind, V, outer, inner, so, si)
     outer, so = 1, 0
     for size, step in zip(reversed(shape[:-2]), reversed(stride[:-2])):
         if size == 1:
@@ -148,6 +151,12 @@ def _distillation(logits, teacher_indices, teacher_logits, labels, temperature, 
     return device, logits, rows, terms, (indices, teacher, labels)
 
 
+def _gradient(logits: torch.Tensor) -> torch.Tensor:
+    if logits.is_contiguous():
+        return torch.empty_like(logits)
+    return torch.empty(*logits.shape, dtype=logits.dtype, device=logits.device)
+
+
 def _launch_distillation(device: int, logits, rows, terms, upstream: Optional[torch.Tensor], grad: Optional[torch.Tensor],
                          stats: Optional[torch.Tensor] = None, want_loss: bool = True) -> Optional[torch.Tensor]:
     """The loss (None where only the gradient is wanted); `stats` [4] receives [sum of the rows' losses, live rows, sum of the hard terms, sum of the divergences]."""
@@ -156,7 +165,7 @@ def _launch_distillation(device: int, logits, rows, terms, upstream: Optional[to
         if stats is not None:
             stats.zero_()
         return torch.zeros((), dtype=torch.float32, device=where)
-    loss = torch.empty((), dtype=torch.float32, device=where) if want_loss else None
+    loss = torch.empty_strided((), (), dtype=torch.float32, device=where) if want_loss else None
     size = _lib.load().gscan_distillation_workspace_bytes(C.byref(rows))
     ws = torch.empty(size, dtype=torch.uint8, device=where)
     _call("gscan_distillation_loss", device, C.byref(rows), C.byref(terms), _lib.ptr(upstream), _lib.ptr(grad), _lib.ptr(loss),
@@ -177,7 +186,7 @@ class _DistillationLoss(torch.autograd.Function):
     def backward(ctx, g):
         logits, indices, teacher, labels = ctx.saved_tensors
         device, logits, rows, terms, _ = _distillation(logits, indices, teacher, labels, *ctx.options)
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        grad = _gradient(logits)
         _launch_distillation(device, logits, rows, terms, g.to(torch.float32).contiguous(), grad, want_loss=False)
         return grad, None, None, None, None
 
@@ -197,7 +206,9 @@ def distillation_loss(logits: torch.Tensor, teacher_indices: torch.Tensor, teach
     labels [...] int64: rows whose label is `ignore_index` or not a word are not live — no loss, a gradient of exactly 0,
     nothing of them is read; without labels every row is live.  `shift_labels`: labels are whole sequences and a row is
     scored against the next one, the last against 0, as `Model.get_loss` does (seq2seq/model.py:108-115).
-    reduction "mean" (0 when no row is live) or "sum".  A differentiable float32 scalar; the gradient goes to `logits` only."""
+    reduction "mean" (0 when no row is live) or "sum".  A differentiable float32 scalar; the gradient goes to `logits` only.
+    Into a graph, capture the backward pass of a loss that was captured too, with no eager loss of the same parameters alive
+    (autograd adds up a parameter's gradient on the stream that it was first used on)."""
     options = (temperature, soft_weight, hard_weight, ignore_index, shift_labels, reduction)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _DistillationLoss.apply(logits, teacher_indices, teacher_logits, labels, options)
@@ -211,28 +222,38 @@ def distillation_loss_and_gradient(logits: torch.Tensor, teacher_indices: torch.
                                    reduction: str = "mean", out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """`distillation_loss` and its gradient with respect to the logits in one pass over them, outside autograd: what a loop
     that issues its own backward pass calls (`train.TrainStep`).  Returns (loss, gradient [..., V] of the logits' type);
-    `out`: a contiguous tensor for the gradient, which may not share memory with the logits."""
+    `out`: a contiguous tensor for the gradient, which may not share memory with an argument."""
     device, logits, rows, terms, _kept = _distillation(logits, teacher_indices, teacher_logits, labels, temperature, soft_weight,
                                                        hard_weight, ignore_index, shift_labels, reduction)
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        out = _gradient(logits)
     else:
-        _check_gradient_out(logits, out)
+        _check_gradient_out(out, logits, _kept)
     return _launch_distillation(device, logits, rows, terms, None, out), out
 
 
-def _check_gradient_out(logits: torch.Tensor, out: torch.Tensor) -> None:
+def _check_gradient_out(out: torch.Tensor, logits: torch.Tensor, others: Sequence[Optional[torch.Tensor]]) -> None:
     _require("logits out", logits, out)
     if out.shape != logits.shape or out.dtype != logits.dtype or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {tuple(logits.shape)} tensor of {logits.dtype}")
-    if _overlap(out, logits):
-        raise ValueError("out shares memory with the logits")
+    if any(t is not None and _overlap(out, t) for t in (logits, *others)):
+        raise ValueError("out shares memory with the logits, the teacher's entries or the labels")
 
 
 def _extent(t: torch.Tensor) -> Tuple[int, int]:
     """First byte and the byte behind the last of a tensor's elements."""
     last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size() if t.numel() else t.data_ptr()
+
+
+def _overlaps_itself(t: torch.Tensor) -> bool:
+    """True unless every element has a place of its own (as far as strides that nest tell)."""
+    end = 1
+    for stride, size in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if stride < end:
+            return True
+        end += (size - 1) * stride
+    return False
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -324,8 +345,9 @@ def beam_reorder(parents: torch.Tensor, states: Union[torch.Tensor, Sequence[tor
                  ) -> Union[torch.Tensor, List[torch.Tensor]]:
     """The beams' states in the order that `beam_select` gave: slice b * W + w of the result is slice b * W + parents[b, w] of
     the state, along `dim` (which has B * W entries).  parents [B, W] int32; states: a tensor of any type, or a sequence of
-    them, all moved in one launch (16 at a time).  `out`: where to write (of the states' shapes, any strides, sharing no
-    memory with them: a slice of a longer cache keeps what lies behind it); otherwise new contiguous tensors are returned.
+    them, all moved in one launch (16 at a time).  `out`: where to write (of the states' shapes, any strides: a slice of a
+    longer cache keeps what lies behind it), in memory whose span, from its first element to its last, meets neither a state's
+    nor another `out`'s; otherwise new contiguous tensors are returned.
     A parent outside [0, W) gives zeros."""
     single = isinstance(states, torch.Tensor)
     sources = [states] if single else list(states)
@@ -341,7 +363,8 @@ def beam_reorder(parents: torch.Tensor, states: Union[torch.Tensor, Sequence[tor
             raise ValueError(f"{len(sources)} states, but {len(targets)} tensors to write them to")
     moves = []
     for i, (s, d) in enumerate(zip(sources, targets)):
-        _require(f"parents states[{i}] out[{i}]", parents, s, d)
+        if s.get_device() != device or d.get_device() != device:
+            _require(f"parents states[{i}] out[{i}]", parents, s, d)
         at = dim + s.dim() if dim < 0 else dim
         if not 0 <= at < s.dim() or s.shape[at] != B * W:
             raise ValueError(f"states[{i}] {tuple(s.shape)} has not {B} x {W} entries along dimension {dim}")
@@ -349,8 +372,11 @@ def beam_reorder(parents: torch.Tensor, states: Union[torch.Tensor, Sequence[tor
             raise ValueError(f"out[{i}] must be {tuple(s.shape)} of {s.dtype}, got {tuple(d.shape)} of {d.dtype}")
         if s.numel() == 0:
             continue
-        if out is not None and any(_overlap(d, other) for other in sources):
-            raise ValueError(f"out[{i}] shares memory with a state")
+        if out is not None:
+            if any(_overlap(d, other) for other in (parents, *sources)):
+                raise ValueError(f"out[{i}] shares memory with a state or with the parents")
+            if _overlaps_itself(d):
+                raise ValueError(f"out[{i}]: elements of {tuple(d.shape)} with the strides {tuple(d.stride())} share memory")
         move = _slices(s, d, at)
         if move is None:
             s = s.contiguous()

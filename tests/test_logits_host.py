@@ -221,3 +221,35 @@ def test_empty_batches_launch_nothing(on_host):
     assert all(t.shape == (0, 4) for t in out)
     assert ops.beam_reorder(torch.zeros(2, 3, dtype=torch.int32), torch.zeros(6, 0)).shape == (6, 0)
     assert not on_host
+
+
+def test_more_threads_than_a_launch_counts_are_refused(lib):
+    """512 threads a row, 256 per four segments of a state: 2^32 of them is more than a launch takes."""
+    many = rows(outer=1 << 23, inner=1, stride_outer=0, stride_inner=0)
+    assert lib.gscan_top_logits(C.byref(many), 3, 4096, 4096, None, None, 0, None) != 0 and "rows" in message(lib)
+    assert lib.gscan_distillation_workspace_bytes(C.byref(many)) == 0 and "rows" in message(lib)
+    many.outer -= 1
+    assert lib.gscan_distillation_workspace_bytes(C.byref(many)) > 0
+    table = (_lib.State * 1)(state(outer=1 << 12, mid=1 << 10, bytes=1 << 13))
+    assert lib.gscan_beam_reorder(2, 3, 4096, table, 1, None) != 0 and "pieces" in message(lib)
+
+
+def test_outputs_that_share_memory_are_refused(on_host):
+    parents, cache = torch.zeros(2, 3, dtype=torch.int32), torch.zeros(6, 4, 5)
+    for out in (torch.zeros(6, 4, 1).expand(6, 4, 5), torch.zeros(1, 4, 5).expand(6, 4, 5), torch.zeros(60).as_strided((6, 4, 5), (8, 4, 1))):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.beam_reorder(parents, cache, out=out)
+    ids = torch.zeros(6, dtype=torch.int32)
+    with pytest.raises(ValueError, match="parents"):
+        ops.beam_reorder(parents, ids, out=parents.view(-1))
+    assert not on_host
+    for out in (torch.zeros(9, 4, 5)[:6], torch.zeros(6, 4, 10)[..., :5], torch.zeros(6, 1, 4, 5)[:, 0]):
+        ops.beam_reorder(parents, cache, out=out)
+    assert len(on_host) == 3
+    x = torch.randn(2, 3, 10)
+    place = torch.zeros(2, 3, 10)
+    teacher = place.view(-1)[:24].view(2, 3, 4)
+    index, labels = torch.zeros(2, 3, 4, dtype=torch.int32), torch.zeros(2, 3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="shares memory"):
+        ops.distillation_loss_and_gradient(x, index, teacher, labels, out=place)
+    assert len(on_host) == 3
