@@ -20,7 +20,7 @@ namespace gscan {
 namespace {
 constexpr int kCountBlocks = 64;
 // Up to so many rows, the launch that needs the number of live rows counts the labels itself, in every workgroup (a launch
-// less: 22.8 for 27.1 us at 5120 rows of 9 words); longer rows fill the chip with workgroups, and theirs come from a launch
+// less: 22.8 for 27.1 us at 5120 rows of 9 words), short rows; long ones fill the chip with workgroups, and theirs come from a launch
 // before them (4088 rows of 32000 words: 134 for 152 us).
 constexpr int kCountThere = 8192, kCountThereLong = 256;
 // Above so many workgroups their parts are added up by 64 workgroups before the one that finishes (rows of 100 words: 8192 rows
@@ -137,6 +137,14 @@ __global__ __launch_bounds__(1024) void distill_finish_kernel(const double *part
     }
 }
 
+// The compiler would keep the widened words, or their exponentials, from one use to the next (twice the registers for 16-bit
+// words, and spills): behind this the pieces are new values to it.
+template <int N>
+__device__ __forceinline__ void hide_pieces(Raw (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(x[i].w[0]), "+v"(x[i].w[1]), "+v"(x[i].w[2]), "+v"(x[i].w[3]));
+}
+
 template <int TPB>
 struct RowShared {
     alignas(16) int index[kMaxTop];
@@ -240,7 +248,7 @@ struct Exponents {
     }
 };
 
-// Rows of 16-byte pieces of 64 words and more, a workgroup per row.
+// Longer rows (group_of, below), a workgroup per row.
 //
 // NR > 0: the row stays in NR pieces per thread.
 // NR = 0: the row is read a second time for the gradient, and its maximum and sums come from one pass in which a thread
@@ -276,13 +284,7 @@ __global__ __launch_bounds__(TPB) __attribute__((amdgpu_waves_per_eu(4))) void d
     for (int i = 0; i < NR; ++i)
         if (has(i)) x[i] = load16<T, true>(row + i * TPB * 16 + at16);
     const float last[1] = {tid < rest ? load1<T>(row, pieces * N + tid) : -INFINITY};
-    // The compiler would keep the widened words from one use to the next (twice the registers for 16-bit words, and
-    // spills): behind this the pieces are new values to it.
-    auto hide = [&]() {
-#pragma unroll
-        for (int i = 0; i < NR; ++i)
-            asm volatile("" : "+v"(x[i].w[0]), "+v"(x[i].w[1]), "+v"(x[i].w[2]), "+v"(x[i].w[3]));
-    };
+    auto hide = [&]() { if constexpr (NR > 0) hide_pieces(x); };
     auto widen = [](const Raw &w, float (&z)[N]) {
 #pragma unroll
         for (int e = 0; e < N; ++e) z[e] = element<T>(w, e);
@@ -490,80 +492,178 @@ __global__ __launch_bounds__(TPB) __attribute__((amdgpu_waves_per_eu(4))) void d
     }
 }
 
-// Vocabularies of at most 64 words: L lanes per row, a word per lane; the teacher's entries of a workgroup's rows in LDS.
-template <class T, int L, bool GRAD>
-__global__ __launch_bounds__(256) void distill_small_kernel(DistillArgs a) {
-    extern __shared__ float entries[];
+// Short rows: L lanes per row, P pieces a lane, 256 / L rows in a workgroup; the reductions stay within a row's lanes and no
+// row waits for another.  The teacher's entries (word, share, the student's logit) lie in LDS; a row's belong to its wave,
+// whose LDS accesses are in order.
+template <int L, class Op>
+__device__ __forceinline__ float group_reduce(float v, Op op) {
+    v = op(v, dpp_move<0xb1, 0xf>(v));                          // quad_perm [1,0,3,2]
+    v = op(v, dpp_move<0x4e, 0xf>(v));                          // quad_perm [2,3,0,1]
+    if constexpr (L > 4) v = op(v, dpp_move<0x141, 0xf>(v));    // row_half_mirror
+    if constexpr (L > 8) v = op(v, dpp_move<0x140, 0xf>(v));    // row_mirror
+    return v;
+}
+
+template <class T, int L, int P, bool GRAD>
+__global__ __launch_bounds__(256) void distill_group_kernel(DistillArgs a, int stride) {
+    extern __shared__ int4 entries[];
     __shared__ float s_part[4][3];
     __shared__ int s_live[4];
-    constexpr int R = 256 / L;
-    const int slot = threadIdx.x / L, v = threadIdx.x & (L - 1), r = blockIdx.x * R + slot, V = a.rows.V, K = a.K;
-    float *share = entries + slot * K;
-    int8_t *index = (int8_t *)(entries + R * K) + slot * K;      // at most 64 words
+    constexpr int R = 256 / L, N = T::vec;
+    const int slot = threadIdx.x / L, lane = threadIdx.x & (L - 1), r = blockIdx.x * R + slot, V = a.rows.V, K = a.K;
+    const int full = V / N, rest = V - full * N;                // whole 16-byte pieces, and words behind them
+    int *index = (int *)entries + slot * stride;                // [R][stride] each
+    float *share = (float *)index + R * stride, *words = share + R * stride;
     const int label = r < a.count ? row_label(a, r) : -1;
-    const bool live = label != -1, in = live && v < V;
+    const bool live = label != -1;
     const char *row = a.rows.row(r < a.count ? r : 0);
-    const float z = in ? load1<T>(row, v) : -INFINITY;
-    auto lanes = [](float x, auto op) {
+    constexpr uint32_t none = __is_same(T, TypeF32) ? 0xff800000u : __is_same(T, TypeBF16) ? 0xff80ff80u : 0xfc00fc00u;      // -inf
+    Raw x[P];
 #pragma unroll
-        for (int d = L / 2; d; d >>= 1) x = op(x, __shfl_xor(x, d, L));
-        return x;
-    };
-    auto larger = [](float x, float y) { return fmaxf(x, y); };
-    auto plus = [](float x, float y) { return x + y; };
-    const float zmax = lanes(z, larger);
-    float tmax = -INFINITY;
-    for (int k = v; k < K; k += L) {
-        const int64_t at = (int64_t)r * K + k;
-        const int i = live ? teacher_index(a, at) : -1;
-        const float t = i >= 0 ? teacher_value(a, at) : -INFINITY;
-        index[k] = (int8_t)i; share[k] = t;
+    for (int i = 0; i < P; ++i) {
+        const int p = lane + i * L;
+        if (live && p < full) x[i] = load16<T, true>(row + (int64_t)p * 16);
+        else if (live && p == full && rest) x[i] = load_tail<T>(row, p * N, V);
+        else x[i] = Raw{{none, none, none, none}};
+    }
+    const float zy = label >= 0 ? load1<T>(row, label) : 0.f;
+    float tmax = -INFINITY, zmax = -INFINITY;
+    for (int k = lane; k < stride; k += L) {
+        int v = -1;
+        float t = -INFINITY, z = 0.f;
+        if (live && k < K) {
+            const int64_t at = (int64_t)r * K + k;
+            v = teacher_index(a, at);
+            if (v >= 0) { t = teacher_value(a, at); z = load1<T>(row, v); }
+        }
+        index[k] = v; share[k] = t; words[k] = z;
         tmax = fmaxf(tmax, t);
     }
-    tmax = lanes(tmax, larger);
-    const bool soft_on = a.soft != 0.f, hard_on = a.hard != 0.f;
-    float A = 0.f, B = 0.f;
-    for (int k = v; k < K; k += L) {
-        const float t = share[k], d = (t - tmax) * a.inv_tau;
-        const int i = index[k];
-        float e = 0.f;
-        if (i >= 0 && t != -INFINITY) {
-            e = __builtin_amdgcn_exp2f(d * kLog2e);
-            if (e != 0.f) { A += e; B += e * (d - (load1<T>(row, i) - zmax) * a.inv_tau); }
+    auto widen = [](const Raw &w, float (&z)[N]) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) z[e] = element<T>(w, e);
+    };
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+#pragma unroll
+        for (int e = 0; e < N; ++e) zmax = fmaxf(zmax, element<T>(x[i], e));
+    auto larger = [](float u, float v) { return fmaxf(u, v); };
+    auto plus = [](float u, float v) { return u + v; };
+    zmax = group_reduce<L>(zmax, larger);
+    tmax = group_reduce<L>(tmax, larger);
+
+    const bool soft_on = a.soft != 0.f, hard_on = a.hard != 0.f, two = soft_on && hard_on && a.inv_tau != 1.f;
+    const float a0 = (soft_on ? a.inv_tau : 1.f) * kLog2e;
+    // the soft term's exponentials, and the hard one's where they differ (`two`)
+    auto exponentials = [&](const float (&z)[N], float (&first)[N], float (&second)[N]) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) first[e] = __builtin_amdgcn_exp2f((z[e] - zmax) * a0);
+        if (!two) return;
+        if (a.power) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) second[e] = first[e] * first[e];
+            if (a.power > 2) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) second[e] *= a.power > 3 ? second[e] : first[e];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) second[e] = __builtin_amdgcn_exp2f((z[e] - zmax) * kLog2e);
         }
+    };
+    float s0 = 0.f, s1 = 0.f, A = 0.f, B = 0.f;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        float z[N], first[N], second[N];
+        widen(x[i], z);
+        exponentials(z, first, second);
+#pragma unroll
+        for (int e = 0; e < N; ++e) s0 += first[e];
+        if (two) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) s1 += second[e];
+        }
+    }
+    for (int k = lane; k < K; k += L) {
+        const float t = share[k], d = (t - tmax) * a.inv_tau;
+        const float e = index[k] >= 0 && t != -INFINITY ? __builtin_amdgcn_exp2f(d * kLog2e) : 0.f;
+        if (e != 0.f) { A += e; B += e * (d - (words[k] - zmax) * a.inv_tau); }
         share[k] = e;
     }
-    // a row's entries stay within its wave, whose LDS accesses are in order: only the compiler has to keep them so
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    A = lanes(A, plus);
-    B = lanes(B, plus);
-    const float e0 = in ? __builtin_amdgcn_exp2f((z - zmax) * a.inv_tau * kLog2e) : 0.f;
-    const float e1 = in ? __builtin_amdgcn_exp2f((z - zmax) * kLog2e) : 0.f;
-    const float s0 = lanes(e0, plus), s1 = lanes(e1, plus);
-    const float zy = label >= 0 ? __shfl(z, label, L) : 0.f;
+    s0 = group_reduce<L>(s0, plus);
+    s1 = two ? group_reduce<L>(s1, plus) : s0;
+    A = group_reduce<L>(A, plus);
+    B = group_reduce<L>(B, plus);
     if constexpr (GRAD) {
         int n = 0;
         if (!a.sum) n = a.live ? a.live[threadIdx.x & 63] : count_live(a, threadIdx.x, 256);
-        n = wave_reduce(n, [](int x, int y) { return x + y; });
+        n = wave_reduce(n, [](int u, int v) { return u + v; });
         if (!a.sum && !a.live) {
             if ((threadIdx.x & 63) == 0) s_live[threadIdx.x >> 6] = n;
             __syncthreads();
             n = s_live[0] + s_live[1] + s_live[2] + s_live[3];
         }
         const float scale = over_live(a, n);
-        float g = 0.f;
-        if (in) {
-            if (hard_on) g = a.hard * scale * (e1 / s1 - (v == label ? 1.f : 0.f));
-            if (soft_on && A != 0.f) {
-                float named = 0.f;
-                for (int k = 0; k < K; ++k) named += index[k] == v ? share[k] : 0.f;
-                g += a.soft_grad * scale * (e0 / s0 - named / A);
+        const float soft = soft_on && A != 0.f ? a.soft_grad * scale : 0.f, hard = hard_on ? a.hard * scale : 0.f;
+        const float c0 = two ? soft / s0 : (soft + hard) / s0, c1 = two ? hard / s1 : 0.f;
+        auto mix = [&](const float (&z)[N], float (&g)[N]) {
+            float first[N], second[N];
+            exponentials(z, first, second);
+#pragma unroll
+            for (int e = 0; e < N; ++e) g[e] = two ? fmaf(c1, second[e], c0 * first[e]) : c0 * first[e];
+        };
+        char *out = a.grad + (int64_t)r * V * T::bytes;
+        hide_pieces(x);
+        if (r < a.count) {
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                const int p = lane + i * L;
+                float z[N], g[N];
+                widen(x[i], z);
+                mix(z, g);
+#pragma unroll
+                for (int e = 0; e < N; ++e) g[e] = live ? g[e] : 0.f;
+                if (p < full) store16<T>(out + (int64_t)p * 16, pack<T>(g));
+                else if (p == full) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e)
+                        if (e < rest) store1<T>(out, p * N + e, g[e]);
+                }
             }
         }
-        if (r < a.count && v < V) store1<T>(a.grad, (int64_t)r * V + v, g);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        // the words that the teacher or the label names, a second time, by the wave that has stored them
+        auto density = [&](float v) {
+            const float d = v - zmax, first = __builtin_amdgcn_exp2f(d * a0);
+            return two ? fmaf(c1, __builtin_amdgcn_exp2f(d * kLog2e), c0 * first) : c0 * first;
+        };
+        const float soft_share = A != 0.f ? soft / A : 0.f;
+        float named_label = 0.f;
+        for (int k = lane; k < K; k += L) {
+            const int v = index[k];
+            if (v < 0) continue;
+            int same = 0;
+            for (int i = 0; i < K; i += 4) {
+                const int4 q = *(const int4 *)&index[i];        // behind K: -1
+                same += (q.x == v) + (q.y == v) + (q.z == v) + (q.w == v);
+            }
+            float named = share[k];
+            bool first = true;
+            if (same > 1) {                                     // left to its first entry, with all of the shares
+                named = 0.f;
+                for (int i = 0; i < K; ++i)
+                    if (index[i] == v) { first = first && i >= k; named += share[i]; }
+            }
+            if (v == label) named_label = 1.f;
+            if (first) store1<T>(out, v, density(words[k]) - soft_share * named - (v == label ? hard : 0.f));
+        }
+        if (hard_on) {
+            named_label = group_reduce<L>(named_label, larger);
+            if (lane == 0 && label >= 0 && named_label == 0.f) store1<T>(out, label, density(zy) - hard);
+        }
     }
     float part[3] = {0.f, 0.f, 0.f};
-    if (live && v == 0) {
+    if (live && lane == 0) {
         part[0] = hard_on ? logf(s1) - (zy - zmax) : 0.f;
         part[1] = soft_on && A != 0.f ? B / A - logf(A) + logf(s0) : 0.f;
         part[2] = 1.f;
@@ -579,19 +679,33 @@ __global__ __launch_bounds__(256) void distill_small_kernel(DistillArgs a) {
                                                         (double)s_part[2][threadIdx.x] + (double)s_part[3][threadIdx.x];
 }
 
-int small_lanes(int V) { return V <= 8 ? 8 : V <= 16 ? 16 : V <= 32 ? 32 : 64; }
-int part_blocks(const gscan_rows &rows) {
+// Rows of up to 8 pieces for each of 16 lanes go to groups of lanes: what a row costs whatever its length (reductions, the
+// teacher's entries, quotients: about 400 instructions of a wave) is then shared by 4 to 16 rows, where a workgroup of one wave
+// per row spends it on each.  262144 rows, loss and gradient / loss alone, against a wave per row: 100 words of float 89 / 47 for
+// 275 / 134 us, 200: 134 / 67 for 296 / 146, 500: 280 / 125 for 379 / 182; of bfloat16 120: 88 / 48 for 300 / 174, 500: 191 / 80
+// for 362 / 233; 32768 rows of 1000: 56 / 24 for 62 / 35.  (A word per lane: 9 words 31 / 16 for 55 / 37, 40 words 72 / 39 for
+// 175 / 134.)  Issue binds them up to some 200 words, the bytes beyond (500 words of float: 3.7 TB/s).
+constexpr int kGroupPieces = 8, kGroupLds = 48 * 1024;
+struct Group { int L, P, stride; };
+bool grouped(const gscan_rows &rows) { return cdiv(rows.V, rows.type == GSCAN_F32 ? 4 : 8) <= 16 * kGroupPieces; }
+Group group_of(const gscan_rows &rows, int K) {
+    const int pieces = cdiv(rows.V, rows.type == GSCAN_F32 ? 4 : 8), stride = (K + 3) & ~3;
+    int L = pieces <= 4 ? 4 : pieces <= 8 ? 8 : 16;
+    while (256 / L * stride * 12 > kGroupLds) L *= 2;           // 16 lanes hold any number of entries
+    return Group{L, cdiv(pieces, L), stride};
+}
+int part_blocks(const gscan_rows &rows, int K) {
     const int64_t n = rows.outer * rows.inner;
-    return rows.V <= 64 ? cdiv(n, 256 / small_lanes(rows.V)) : (int)n;
+    return grouped(rows) ? cdiv(n, 256 / group_of(rows, K).L) : (int)n;
 }
 
-template <class T, int L>
-int launch_small(const DistillArgs &a, hipStream_t stream) {
-    const int blocks = cdiv(a.count, 256 / L);
-    const size_t lds = (size_t)(256 / L) * a.K * 5;
-    if (a.grad) hipLaunchKernelGGL((distill_small_kernel<T, L, true>), dim3(blocks), dim3(256), lds, stream, a);
-    else hipLaunchKernelGGL((distill_small_kernel<T, L, false>), dim3(blocks), dim3(256), lds, stream, a);
-    GSCAN_LAUNCHED("distill_small_kernel");
+template <class T, int L, int P>
+int launch_group(const DistillArgs &a, int stride, hipStream_t stream) {
+    const dim3 grid(cdiv(a.count, 256 / L)), block(256);
+    const size_t lds = (size_t)(256 / L) * stride * 12;
+    if (a.grad) hipLaunchKernelGGL((distill_group_kernel<T, L, P, true>), grid, block, lds, stream, a, stride);
+    else hipLaunchKernelGGL((distill_group_kernel<T, L, P, false>), grid, block, lds, stream, a, stride);
+    GSCAN_LAUNCHED("distill_group_kernel");
     return 0;
 }
 
@@ -607,15 +721,16 @@ int launch_row(const DistillArgs &a, hipStream_t stream) {
 }
 
 template <class T>
-int launch_type(const DistillArgs &a, hipStream_t stream) {
+int launch_type(const DistillArgs &a, const gscan_rows &rows, hipStream_t stream) {
     const int V = a.rows.V;
-    if (V <= 64) {
-        switch (small_lanes(V)) {
-            case 8: return launch_small<T, 8>(a, stream);
-            case 16: return launch_small<T, 16>(a, stream);
-            case 32: return launch_small<T, 32>(a, stream);
-            default: return launch_small<T, 64>(a, stream);
-        }
+    if (grouped(rows)) {
+        const Group g = group_of(rows, a.K);
+        if (g.L == 4) return launch_group<T, 4, 1>(a, g.stride, stream);
+        if (g.L == 8) return launch_group<T, 8, 1>(a, g.stride, stream);
+        if (g.P == 1) return launch_group<T, 16, 1>(a, g.stride, stream);
+        if (g.P == 2) return launch_group<T, 16, 2>(a, g.stride, stream);
+        if (g.P <= 4) return launch_group<T, 16, 4>(a, g.stride, stream);
+        return launch_group<T, 16, 8>(a, g.stride, stream);
     }
     const int pieces = V / T::vec;
     if (!a.grad) {
@@ -631,7 +746,7 @@ int launch_type(const DistillArgs &a, hipStream_t stream) {
 }  // namespace
 
 size_t distillation_workspace(const gscan_rows &rows) {
-    return kCountBlocks * (sizeof(int) + 3 * sizeof(double)) + (size_t)part_blocks(rows) * 3 * sizeof(double);
+    return kCountBlocks * (sizeof(int) + 3 * sizeof(double)) + (size_t)(grouped(rows) ? cdiv(rows.outer * rows.inner, 16) : rows.outer * rows.inner) * 3 * sizeof(double);
 }
 
 int distillation_loss(const gscan_rows &rows, const gscan_distillation &t, const float *upstream, void *grad, float *loss,
@@ -664,19 +779,19 @@ int distillation_loss(const gscan_rows &rows, const gscan_distillation &t, const
     double *sums = (double *)(live + kCountBlocks);
     a.part = sums + 3 * kCountBlocks;
     a.sum = t.sum_reduction != 0;
-    if (grad && !a.sum && a.count > (rows.V <= 64 ? kCountThere : kCountThereLong)) {       // the gradient of a mean needs the number of live rows first
+    if (grad && !a.sum && a.count > (grouped(rows) ? kCountThere : kCountThereLong)) {       // the gradient of a mean needs the number of live rows first
         a.live = live;
         hipLaunchKernelGGL(distill_count_kernel, dim3(kCountBlocks), dim3(256), 0, stream, a, live);
         GSCAN_LAUNCHED("distill_count_kernel");
     }
     const int type = rows.type;
-    TRY_RC(type == GSCAN_F32    ? launch_type<TypeF32>(a, stream)
-           : type == GSCAN_BF16 ? launch_type<TypeBF16>(a, stream)
-                                : launch_type<TypeF16>(a, stream));
+    TRY_RC(type == GSCAN_F32    ? launch_type<TypeF32>(a, rows, stream)
+           : type == GSCAN_BF16 ? launch_type<TypeBF16>(a, rows, stream)
+                                : launch_type<TypeF16>(a, rows, stream));
     if (!loss) return 0;
     const float tau2 = t.temperature * t.temperature;
     const double *part = a.part;
-    int parts = part_blocks(rows);
+    int parts = part_blocks(rows, t.K);
     if (parts > kFinishParts) {
         hipLaunchKernelGGL(distill_add_kernel, dim3(kCountBlocks), dim3(256), 0, stream, part, parts, sums);
         GSCAN_LAUNCHED("distill_add_kernel");

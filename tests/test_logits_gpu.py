@@ -207,6 +207,50 @@ def test_distillation_matches_its_formula(ops, dtype, lead, V, K, options):
     assert torch.equal(ops.distillation_loss_and_gradient(zd, idd, td, yd, **kw)[1], got)       # the same bits again
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lead,V,K", [((67,), 5, 3), ((40,), 9, 100), ((35,), 9, 130), ((33,), 31, 70), ((18,), 33, 2), ((17,), 129, 130),
+                                      ((5, 3), 257, 9), ((17,), 511, 1), ((3,), 513, 33), ((18,), 1023, 7), ((3,), 1025, 5)])
+def test_distillation_of_short_rows(ops, dtype, lead, V, K):
+    """Rows that share a wave with others (up to 512 words of 32 bits, 1024 of 16) and those just behind; the last workgroup
+    has fewer rows than places, some of its rows are not live, more entries than words."""
+    for options in (1, 2, 5):
+        kw = dict(OPTIONS[options], ignore_index=0)
+        z, index, teacher, labels = student(lead, V, K, dtype, options + 70, (torch.int64, torch.int32)[options % 2])
+        labels.view(-1)[1::3] = 0
+        want, grad, size = distill_oracle(z, index, teacher, labels, **kw)
+        zd, idd, td, yd = z.cuda(), index.cuda(), teacher.cuda(), labels.cuda()
+        loss, got = ops.distillation_loss_and_gradient(zd, idd, td, yd, **kw)
+        rows = 1 if kw.get("reduction") != "sum" else labels.numel()
+        weight = kw.get("soft_weight", 1.0) * kw.get("temperature", 1.0) ** 2 + kw.get("hard_weight", 0.0)
+        check_loss(loss, want, rows * weight * (2 + math.log(V)))
+        check_gradient(got, grad, size, dtype)
+        assert (got.cpu()[labels == 0] == 0).all()
+        check_loss(ops.distillation_loss(zd, idd, td, yd, **kw), want, rows * weight * (2 + math.log(V)))
+
+
+@pytest.mark.parametrize("n,V", [(8193, 1030), (131200, 70)])
+def test_sums_of_many_rows(ops, n, V):
+    """More workgroups than one launch adds up; the mean is counted by a launch of its own."""
+    g = gen(n, V)
+    z, labels = torch.randn(n, V, generator=g), torch.randint(0, V, (n,), generator=g)
+    index = torch.stack([labels, (labels + 1) % V], 1).int()
+    teacher = torch.randn(n, 2, generator=g)
+    live = labels != 0
+    logp, logq, logs = (torch.log_softmax(t.double(), -1) for t in (teacher / 2, z / 2, z))
+    rows = 0.5 * 4 * (logp.exp() * (logp - logq.gather(1, index.long()))).sum(1) - 0.25 * logs.gather(1, labels[:, None])[:, 0]
+    want = rows[live].mean().item()
+    kw = dict(temperature=2.0, soft_weight=0.5, hard_weight=0.25, ignore_index=0)
+    loss, got = ops.distillation_loss_and_gradient(z.cuda(), index.cuda(), teacher.cuda(), labels.cuda(), **kw)
+    check_loss(loss, want, 2.25 * (2 + math.log(V)))
+    check_loss(ops.distillation_loss(z.cuda(), index.cuda(), teacher.cuda(), labels.cuda(), **kw), want, 2.25 * (2 + math.log(V)))
+    target = torch.zeros(n, V, dtype=torch.float64).scatter_(1, index.long(), logp.exp())
+    pick = torch.zeros(n, V, dtype=torch.float64).scatter_(1, labels[:, None], 1.0)
+    scale = live.double()[:, None] / live.sum()
+    check_gradient(got, scale * (logq.exp() - target + 0.25 * (logs.exp() - pick)),
+                   scale * (logq.exp() + target + 0.25 * (logs.exp() + pick)), torch.float32)
+    assert (got.cpu()[~live] == 0).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("V", [66000, 131075])
 def test_distillation_over_large_vocabularies(ops, dtype, V):
