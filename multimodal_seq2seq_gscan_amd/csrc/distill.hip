@@ -495,15 +495,6 @@ __global__ __launch_bounds__(TPB) __attribute__((amdgpu_waves_per_eu(4))) void d
 // Short rows: L lanes per row, P pieces a lane, 256 / L rows in a workgroup; the reductions stay within a row's lanes and no
 // row waits for another.  The teacher's entries (word, share, the student's logit) lie in LDS; a row's belong to its wave,
 // whose LDS accesses are in order.
-template <int L, class Op>
-__device__ __forceinline__ float group_reduce(float v, Op op) {
-    v = op(v, dpp_move<0xb1, 0xf>(v));                          // quad_perm [1,0,3,2]
-    v = op(v, dpp_move<0x4e, 0xf>(v));                          // quad_perm [2,3,0,1]
-    if constexpr (L > 4) v = op(v, dpp_move<0x141, 0xf>(v));    // row_half_mirror
-    if constexpr (L > 8) v = op(v, dpp_move<0x140, 0xf>(v));    // row_mirror
-    return v;
-}
-
 template <class T, int L, int P, bool GRAD>
 __global__ __launch_bounds__(256) void distill_group_kernel(DistillArgs a, int stride) {
     extern __shared__ int4 entries[];

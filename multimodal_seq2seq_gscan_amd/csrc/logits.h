@@ -187,6 +187,34 @@ __device__ __forceinline__ V wave_reduce(V v, Op op) {
     return v;
 }
 
+// The same over groups of L = 4, 8 or 16 lanes, on the DPP datapath.  All lanes must be active.
+template <int CTRL, typename V>
+__device__ __forceinline__ V dpp_word(V v) {
+    static_assert(sizeof(V) == 4, "a word");
+    int w;
+    __builtin_memcpy(&w, &v, 4);
+    w = __builtin_amdgcn_update_dpp(0, w, CTRL, 0xf, 0xf, false);
+    __builtin_memcpy(&v, &w, 4);
+    return v;
+}
+template <int L, typename V, class Op>
+__device__ __forceinline__ V group_reduce(V v, Op op) {
+    v = op(v, dpp_word<0xb1>(v));                          // quad_perm [1,0,3,2]
+    v = op(v, dpp_word<0x4e>(v));                          // quad_perm [2,3,0,1]
+    if constexpr (L > 4) v = op(v, dpp_word<0x141>(v));    // row_half_mirror
+    if constexpr (L > 8) v = op(v, dpp_word<0x140>(v));    // row_mirror
+    return v;
+}
+// how many of the sixteen lanes' numbers come before this lane's
+__device__ __forceinline__ int sum_before16(int v) {
+    int s = v;
+    s += dpp_word<0x111>(s);                               // row_shr:1, 2, 4, 8: 0 from outside the row
+    s += dpp_word<0x112>(s);
+    s += dpp_word<0x114>(s);
+    s += dpp_word<0x118>(s);
+    return s - v;
+}
+
 // log sum exp from the parts of a row's chunks, in 64 bits; one wave.
 __device__ __forceinline__ double join_lse(const LsePart *part, int n) {
     const int lane = threadIdx.x & 63;
@@ -202,12 +230,13 @@ __device__ __forceinline__ double join_lse(const LsePart *part, int n) {
 // A number t such that at least K of n keys in LDS are >= t, and (unless many are equal) few more than K: bisection between
 // the keys' least and largest, counting with ballots; it ends as soon as the count is within K .. K + K/4, or the interval is
 // one number.  One wave, n <= 64 * SLOTS.  With fewer than K keys > 0 the answer is 0.
-template <int SLOTS>
-__device__ __forceinline__ uint32_t kth_bound(const uint32_t *keys, int n, int K, int lane) {
+// `keys(i)` reads the i-th.
+template <int SLOTS, class F>
+__device__ __forceinline__ uint32_t kth_bound(F keys, int n, int K, int lane) {
     uint32_t k[SLOTS], hi = 0, lo = ~0u;
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i) {
-        k[i] = lane + 64 * i < n ? keys[lane + 64 * i] : 0u;
+        k[i] = lane + 64 * i < n ? keys(lane + 64 * i) : 0u;
         hi = max(hi, k[i]);
         if (k[i]) lo = min(lo, k[i]);
     }

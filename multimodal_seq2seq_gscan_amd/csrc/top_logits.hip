@@ -19,6 +19,7 @@ namespace gscan {
 
 namespace {
 constexpr int kHits = 1024;        // groups of pieces that reach the bound
+constexpr int kGroupList = 96;     // words of a short row that reach the bound
 
 struct TopArgs {
     Rows rows;
@@ -216,7 +217,8 @@ __device__ int find_candidates(const S &src, Sh &sh, int K, F scan) {
     if (tid < 64) {
         // K of TPB maxima bound nearly as well as K of four times as many, for a quarter of the counting, while K is no more
         // than a quarter of them
-        const uint32_t b = 4 * K <= TPB ? kth_bound<TPB / 64>(sh.thread_keys, TPB, K, tid) : kth_bound<4 * TPB / 64>(sh.keys, 4 * TPB, K, tid);
+        const uint32_t b = 4 * K <= TPB ? kth_bound<TPB / 64>([&](int i) { return sh.thread_keys[i]; }, TPB, K, tid)
+                                        : kth_bound<4 * TPB / 64>([&](int i) { return sh.keys[i]; }, 4 * TPB, K, tid);
         if (tid == 0) { sh.bound = b; sh.hits = 0; sh.count = 0; }
     }
     __syncthreads();
@@ -310,6 +312,20 @@ __device__ __forceinline__ void put_out(const TopArgs &a, int64_t at, uint64_t x
     a.indices[at] = pair_index(x);
 }
 
+// The maxima of a piece's quarters, as ordered numbers; 0 without a piece.  (Words behind the row's end are -inf: a bound that
+// they take part in is -inf, which every word reaches.)
+template <class T>
+__device__ __forceinline__ void quarters(const Raw &x, bool there, uint32_t (&q)[4]) {
+    constexpr int Q = T::vec / 4;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        float t = element<T>(x, u * Q);
+#pragma unroll
+        for (int e = 1; e < Q; ++e) t = fmaxf(t, element<T>(x, u * Q + e));
+        q[u] = there ? order_key(t) : 0u;
+    }
+}
+
 // One workgroup per row, or per chunk of a row.  PIECES = 0: at most four pieces a thread, which stay in registers: nothing is
 // read again.
 template <class T, int TPB, bool LSE, int PIECES>
@@ -392,14 +408,32 @@ __global__ __launch_bounds__(TPB) void top_row_kernel(TopArgs a) {
         if (k) { sh.piece[s * TPB + tid] = (uint16_t)(order_key(group) >> 16); ++s; }
         for (; s < groups; ++s) sh.piece[s * TPB + tid] = 0;
     }
-    uint32_t most = 0;
+    uint32_t most = 0, four[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-        const uint32_t k = tid + u * TPB < pieces ? order_key(top[u]) : 0u;
-        if (4 * a.K > TPB) sh.keys[u * TPB + tid] = k;
-        most = max(most, k);
+        four[u] = tid + u * TPB < pieces ? order_key(top[u]) : 0u;
+        most = max(most, four[u]);
     }
     sh.thread_keys[tid] = most;
+    if (4 * a.K > TPB) {
+        if constexpr (PIECES == 0) {
+            // one or two pieces a thread: maxima of quarters or halves of them, or a large K is bounded by hardly more than
+            // the least of the maxima, and most words reach that (2000 bfloat16 words, K = 200: 777 for 135 us, 16384 rows)
+            if (pieces <= TPB) {
+                quarters<T>(held[0], tid < pieces, four);
+            } else if (pieces <= 2 * TPB) {
+                uint32_t q[4];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    quarters<T>(held[u], tid + u * TPB < pieces, q);
+                    four[2 * u] = max(q[0], q[1]);
+                    four[2 * u + 1] = max(q[2], q[3]);
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sh.keys[u * TPB + tid] = four[u];
+    }
 
     if constexpr (LSE) {
         if (sum.sum != sum.sum) {          // a NaN among the words (or an infinity): they count as -inf
@@ -530,7 +564,136 @@ __global__ __launch_bounds__(TPB) void top_join_kernel(TopArgs a) {
     rank_candidates<TPB>(sh, n, a.K, [&](int place, uint64_t x) { put_out<T>(a, (int64_t)r * a.K + place, x); });
 }
 
-// Vocabularies of at most 64 words: L lanes per row, a word per lane, a word's place counted against the other lanes'.
+// Short rows, few words looked for: sixteen lanes per row, P pieces a lane, held as numbers (a NaN behind the row's end, where
+// no comparison is true).  A bound that K words reach comes from bisection, counting the pieces' maxima, or the words where a
+// row has few pieces; the words that reach it go to a list in LDS and are ranked by counting.  Where more reach it than the
+// list takes (many words alike), the K best are taken out one by one.  A row stays within its lanes: nothing waits at a barrier.
+template <class T, int P, bool LSE>
+__global__ __launch_bounds__(256) void top_group_kernel(TopArgs a, int rows) {
+    constexpr int R = 16, N = T::vec, W = P * N;
+    __shared__ alignas(16) uint64_t s_list[R][kGroupList + 2];
+    const int slot = threadIdx.x >> 4, lane = threadIdx.x & 15, r = blockIdx.x * R + slot, V = a.rows.V, K = a.K;
+    const bool live = r < rows && !(a.finished && (a.finished[r] || a.scores[r] == -INFINITY));
+    const char *row = a.rows.row(r < rows ? r : 0);
+    const int full = V / N, rest = V - full * N, pieces = full + (rest ? 1 : 0);
+    uint64_t *list = s_list[slot];
+    float z[W], most[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const int p = lane + i * 16;
+        Raw x{{0, 0, 0, 0}};
+        if (live && p < full) x = load16<T, true>(row + (int64_t)p * 16);
+        else if (live && p == full && rest) x = load_tail<T>(row, p * N, V);
+        const int words = !live ? 0 : p < full ? N : p == full ? rest : 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) z[i * N + e] = e < words ? fmaxf(element<T>(x, e), -INFINITY) : NAN;
+    }
+    float lowest = NAN, zmax = NAN;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        most[i] = z[i * N];
+#pragma unroll
+        for (int e = 1; e < N; ++e) most[i] = fmaxf(most[i], z[i * N + e]);
+        lowest = fminf(lowest, most[i]);
+        zmax = fmaxf(zmax, most[i]);
+    }
+    lowest = group_reduce<16>(lowest, [](float u, float v) { return fminf(u, v); });
+    zmax = group_reduce<16>(zmax, [](float u, float v) { return fmaxf(u, v); });
+    auto plus = [](int u, int v) { return u + v; };
+    auto index_of = [&](int i) { return (lane + i / N * 16) * N + i % N; };
+
+    // count(>= lo) >= K and count(>= top) < K, of what is counted
+    const bool by_piece = pieces >= 2 * K;
+    uint32_t lo = pieces >= K ? order_key(lowest) : 0x007fffffu, top = order_key(zmax) + 1;
+    bool found = !live || top - lo <= 1;
+    while (__ballot(!found)) {
+        const uint32_t mid = lo + (top - lo) / 2;
+        const float v = key_value(mid);
+        int c = 0;
+        if (by_piece) {
+#pragma unroll
+            for (int i = 0; i < P; ++i) c += most[i] >= v ? 1 : 0;
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) c += z[i] >= v ? 1 : 0;
+        }
+        c = group_reduce<16>(c, plus);
+        if (!found) {
+            if (c >= K) { lo = mid; found = c <= K + (K >> 2); }
+            else top = mid;
+            found = found || top - lo <= 1;
+        }
+    }
+    const float bound = key_value(lo);
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) mine += z[i] >= bound ? 1 : 0;
+    const int n = group_reduce<16>(mine, plus);
+    int at = sum_before16(mine);
+    const bool fits = n <= kGroupList;
+    auto put = [&](int place, uint64_t x) {
+        if (a.keys) a.keys[(int64_t)r * K + place] = x;
+        else put_out<T>(a, (int64_t)r * K + place, x);
+    };
+    if (fits) {
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+            if (z[i] >= bound) list[at++] = (uint64_t)__float_as_uint(z[i]) << 32 | (uint32_t)index_of(i);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int i = lane; i < n; i += 16) {
+            const uint64_t x = list[i];
+            list[i] = pair_key(order_key(__uint_as_float((uint32_t)(x >> 32))), (int)(uint32_t)x);
+        }
+        if (lane == 0) list[n] = 0;                        // a pair is compared at a time
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int i = lane; i < n; i += 16) {
+            const uint64_t x = list[i];
+            const double me = pair_double(x);
+            int place = 0;
+            for (int j = 0; j < n; j += 2) {
+                const double2 q = *(const double2 *)&list[j];
+                place += (q.x > me ? 1 : 0) + (q.y > me ? 1 : 0);
+            }
+            if (place < K) put(place, x);
+        }
+    }
+    if constexpr (LSE) {
+        const float m = fmaxf(zmax, -FLT_MAX);
+        double sum = 0.0;                                  // of a piece in 32 bits, from there on in 64
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            float s = 0.f;
+#pragma unroll
+            for (int e = i * N; e < i * N + N; ++e) s += z[e] == z[e] ? __builtin_amdgcn_exp2f((z[e] - m) * kLog2e) : 0.f;
+            sum += s;
+        }
+#pragma unroll
+        for (int k = 8; k; k >>= 1) sum += __shfl_xor(sum, k);
+        if (live && lane == 0) {
+            if (a.parts) a.parts[r] = LsePart{sum, m, 0.f};
+            else a.lse[r] = m == INFINITY ? INFINITY : (float)((double)m + log(sum));
+        }
+    }
+    if (__ballot(!fits)) {
+        for (int place = 0; place < K; ++place) {
+            float best = NAN;
+            int which = 0x7fffffff;
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+                if (z[i] > best || (best != best && z[i] == z[i])) { best = z[i]; which = index_of(i); }
+            const float all = group_reduce<16>(best, [](float u, float v) { return fmaxf(u, v); });
+            const int first = group_reduce<16>(best == all ? which : 0x7fffffff, [](int u, int v) { return min(u, v); });
+            if (!fits && first == which && best == all) {
+                put(place, pair_key(order_key(best), first));
+#pragma unroll
+                for (int i = 0; i < W; ++i)
+                    if (index_of(i) == first) z[i] = NAN;
+            }
+        }
+    }
+}
+
+// Vocabularies of at most 16 words: L lanes per row, a word per lane, a word's place counted against the other lanes'.
 template <class T, int L>
 __global__ __launch_bounds__(256) void top_small_kernel(TopArgs a, int rows) {
     const int r = blockIdx.x * (256 / L) + threadIdx.x / L, v = threadIdx.x & (L - 1);
@@ -552,6 +715,14 @@ __global__ __launch_bounds__(256) void top_small_kernel(TopArgs a, int rows) {
     }
 }
 
+// Short rows share a wave.  262144 rows against a wave per row (a word per lane up to 64 words): 20 words of float, K = 4: 42 for
+// 86 us, 64 words: 46 for 335; 131072 rows, K = 4 / 32: 100 words of float 31 / 56 for 132 / 217, 200: 41 / 73 for 135 / 180, of
+// bfloat16 500: 58 / 104 for 162 / 213; 65536 rows of 1000: 57 / 90 for 74 / 97.  Issue binds them; 9 words are faster a word per
+// lane (25 for 43).
+bool top_grouped(const gscan_rows &rows, int K) {
+    return K <= 64 && rows.V > 16 && cdiv(rows.V, rows.type == GSCAN_F32 ? 4 : 8) <= 16 * 8;
+}
+
 // A wave per row where a wave's 256 groups suffice for K and a row is short: no barrier is waited at.
 bool one_wave(const gscan_rows &rows, int K) { return K <= 64 && rows.V <= 2048; }
 
@@ -568,8 +739,8 @@ template <class T, int TPB>
 int launch_rows(const TopArgs &a, int64_t grid, bool lse, hipStream_t stream) {
     const int pieces = cdiv(a.chunk, T::vec);
     if (pieces <= 4 * TPB) return launch_rows<T, TPB, 0>(a, grid, lse, stream);
-    if (pieces <= 16 * TPB) return launch_rows<T, TPB, 16 * TPB>(a, grid, lse, stream);
-    return launch_rows<T, TPB, 32 * TPB>(a, grid, lse, stream);
+    if (TPB == 64 || pieces <= 16 * TPB) return launch_rows<T, TPB, 16 * TPB>(a, grid, lse, stream);      // a wave: 2048 words at most
+    return launch_rows<T, 256, 32 * 256>(a, grid, lse, stream);
 }
 template <class T>
 int launch_rows(const TopArgs &a, int64_t grid, bool lse, bool wave, hipStream_t stream) {
@@ -580,11 +751,26 @@ template <class T>
 int launch_small(const TopArgs &a, int rows, hipStream_t stream) {
     const int V = a.rows.V;
     if (V <= 8) hipLaunchKernelGGL((top_small_kernel<T, 8>), dim3(cdiv(rows, 32)), dim3(256), 0, stream, a, rows);
-    else if (V <= 16) hipLaunchKernelGGL((top_small_kernel<T, 16>), dim3(cdiv(rows, 16)), dim3(256), 0, stream, a, rows);
-    else if (V <= 32) hipLaunchKernelGGL((top_small_kernel<T, 32>), dim3(cdiv(rows, 8)), dim3(256), 0, stream, a, rows);
-    else hipLaunchKernelGGL((top_small_kernel<T, 64>), dim3(cdiv(rows, 4)), dim3(256), 0, stream, a, rows);
+    else hipLaunchKernelGGL((top_small_kernel<T, 16>), dim3(cdiv(rows, 16)), dim3(256), 0, stream, a, rows);
     GSCAN_LAUNCHED("top_small_kernel");
     return 0;
+}
+
+template <class T, int P>
+int launch_group(const TopArgs &a, int rows, bool lse, hipStream_t stream) {
+    const dim3 grid(cdiv(rows, 16));
+    if (lse) hipLaunchKernelGGL((top_group_kernel<T, P, true>), grid, dim3(256), 0, stream, a, rows);
+    else hipLaunchKernelGGL((top_group_kernel<T, P, false>), grid, dim3(256), 0, stream, a, rows);
+    GSCAN_LAUNCHED("top_group_kernel");
+    return 0;
+}
+template <class T>
+int launch_group(const TopArgs &a, int rows, bool lse, hipStream_t stream) {
+    const int pieces = cdiv(a.rows.V, T::vec);
+    if (pieces <= 16) return launch_group<T, 1>(a, rows, lse, stream);
+    if (pieces <= 32) return launch_group<T, 2>(a, rows, lse, stream);
+    if (pieces <= 64) return launch_group<T, 4>(a, rows, lse, stream);
+    return launch_group<T, 8>(a, rows, lse, stream);
 }
 
 template <class T>
@@ -630,6 +816,10 @@ int top_chunk_keys(const gscan_rows &rows, int K, TopChunks c, uint64_t *keys, L
     a.K = K; a.splits = c.splits; a.chunk = c.chunk;
     a.keys = keys; a.parts = parts; a.finished = finished; a.scores = scores;
     const int64_t grid = rows.outer * rows.inner * c.splits;
+    if (top_grouped(rows, K))
+        return BY_TYPE(rows.type, launch_group<TypeF32>(a, (int)grid, parts != nullptr, stream),
+                       launch_group<TypeBF16>(a, (int)grid, parts != nullptr, stream),
+                       launch_group<TypeF16>(a, (int)grid, parts != nullptr, stream));
     const bool wave = one_wave(rows, K);
     return BY_TYPE(rows.type, launch_rows<TypeF32>(a, grid, parts != nullptr, wave, stream),
                    launch_rows<TypeBF16>(a, grid, parts != nullptr, wave, stream),
@@ -637,7 +827,6 @@ int top_chunk_keys(const gscan_rows &rows, int K, TopChunks c, uint64_t *keys, L
 }
 
 size_t top_logits_workspace(const gscan_rows &rows, int K) {
-    if (rows.V <= 64) return 0;
     const TopChunks c = top_chunks(rows, K);
     return c.splits == 1 ? 0 : (size_t)(rows.outer * rows.inner) * c.splits * (K * sizeof(uint64_t) + sizeof(LsePart));
 }
@@ -650,7 +839,10 @@ int top_logits(const gscan_rows &rows, int K, void *values, int32_t *indices, fl
     TopArgs a{};
     a.rows = device_rows(rows);
     a.K = K; a.values = values; a.indices = indices; a.lse = lse;
-    if (rows.V <= 64)
+    if (top_grouped(rows, K))
+        return BY_TYPE(rows.type, launch_group<TypeF32>(a, n, lse != nullptr, stream), launch_group<TypeBF16>(a, n, lse != nullptr, stream),
+                       launch_group<TypeF16>(a, n, lse != nullptr, stream));
+    if (rows.V <= 16)
         return BY_TYPE(rows.type, launch_small<TypeF32>(a, n, stream), launch_small<TypeBF16>(a, n, stream),
                        launch_small<TypeF16>(a, n, stream));
     const TopChunks c = top_chunks(rows, K);

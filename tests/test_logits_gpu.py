@@ -91,6 +91,24 @@ def test_top_of_awkward_rows(ops, dtype, rows, V, k):
         check_top(ops, torch.sort(x, dim=-1, descending=order)[0].cuda(), k)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,V,k", [(19, 65, 32), (16, 100, 1), (5, 127, 20), (33, 128, 4), (7, 129, 16), (17, 256, 32), (3, 257, 5),
+                                      (18, 500, 31), (2, 512, 33), (35, 513, 8), (17, 1000, 32), (5, 1024, 2), (3, 1025, 32), (3, 700, 100), (5, 2000, 200), (2, 2100, 256),
+                                      (3, 4000, 256)])
+def test_top_of_short_rows(ops, dtype, rows, V, k):
+    """Rows that share a wave with others (up to 512 words of 32 bits, 1024 of 16, at most 64 looked for) and those behind; many looked
+    for among few pieces."""
+    test_top_matches_a_stable_sort(ops, dtype, rows, V, k)
+    test_top_of_awkward_rows(ops, dtype, rows, V, k)
+    x = torch.zeros(rows, V)                               # a few above many equal ones, in some of the rows
+    x[::2, V // 3:V // 3 + min(5, k)] = 7.0
+    x[1::2] = torch.randn(rows, V, generator=gen(rows, V, 3))[1::2]
+    check_top(ops, x.to(dtype).cuda(), k)
+    values, index = ops.top_logits(x.to(dtype).cuda()[:, 1:][::3], min(k, V - 1))       # strided, any alignment
+    want = top_oracle(x.to(dtype)[:, 1:][::3], min(k, V - 1))
+    assert torch.equal(index.cpu().long(), want[1]) and torch.equal(values.cpu().double(), want[0])
+
+
 @pytest.mark.parametrize("dtype,k", [(torch.float32, 256), (torch.bfloat16, 256), (torch.float16, 100)])
 def test_top_of_rows_laid_out_against_the_grouping(ops, dtype, k):
     """Rows whose large words share the threads that keep one maximum each: more candidates than the list holds."""
