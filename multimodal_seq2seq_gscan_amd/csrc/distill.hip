@@ -7,8 +7,9 @@
 // A row is read once: it stays in registers, as it came (16-byte pieces), between the two reductions (its maximum, its sums)
 // and the gradient.  The exponentials are taken a second time for the gradient: holding them would take twice the registers
 // for 16-bit words.  sum_k p_k (log p_k - log q_k) needs no normalisers inside: with e_k = exp((t_k - t_max) / tau) and
-// A = sum e, B = sum e_k ((t_k - t_max) - (z_k - z_max)) / tau it is B / A - log A + log sum exp((z - z_max) / tau), so
-// one more reduction beside the row's sums does it.  Sums are in 32 bits within a row and in 64 across rows.
+// A = sum e, B = sum e_k ((t_k - t_max) - (z_k - z_max)) it is B / (A tau) + log(sum exp((z - z_max) / tau) / A), so
+// one more reduction beside the row's sums does it; the same rounded 1 / tau stands in p, q and B: it changes the temperature,
+// not the difference.  Sums are in 32 bits within a row and in 64 across rows.
 // The few words that the teacher or the label names are stored a second time behind the row, with their share taken off:
 // same workgroup, behind a barrier; an index that comes twice is handled once, by its first entry, with both shares.
 #include <type_traits>
@@ -393,11 +394,11 @@ __global__ __launch_bounds__(TPB) __attribute__((amdgpu_waves_per_eu(4))) void d
 #pragma unroll
     for (int j = 0; j < NK; ++j) {
         const int k = tid + j * TPB;
-        const float d = (t[j] - tmax) * a.inv_tau;
-        share[j] = idx[j] >= 0 && t[j] != -INFINITY ? __builtin_amdgcn_exp2f(d * kLog2e) : 0.f;
+        const float d = t[j] - tmax;
+        share[j] = idx[j] >= 0 && t[j] != -INFINITY ? __builtin_amdgcn_exp2f(d * a0) : 0.f;
         if (share[j] != 0.f) {
             sums[2] += share[j];
-            sums[3] += share[j] * (d - (zk[j] - zmax) * a.inv_tau);
+            sums[3] += share[j] * (d - (zk[j] - zmax));
         }
         if (GRAD && k < a.K) sh.share[k] = share[j];
     }
@@ -408,7 +409,7 @@ __global__ __launch_bounds__(TPB) __attribute__((amdgpu_waves_per_eu(4))) void d
         const float off0 = near ? fmaf(zmax, a0, b0) * 0.6931471805599453f : 0.f;
         const float off1 = E == kPower ? off0 * (float)a.power : E == kTwo && near ? fmaf(zmax, a1, b1) * 0.6931471805599453f : off0;
         part[0] = a.hard != 0.f ? (double)(logf(s1) - off1 - (zy - zmax)) : 0.0;
-        part[1] = a.soft != 0.f && A != 0.f ? (double)(B / A - logf(A) + (logf(s0) - off0)) : 0.0;
+        part[1] = a.soft != 0.f && A != 0.f ? (double)B / A * (a0 * 0.6931471805599453) + log((double)s0 / A) - off0 : 0.0;
         part[2] = 1.0;
     }
     if constexpr (GRAD) {
@@ -498,9 +499,9 @@ __global__ __launch_bounds__(TPB) __attribute__((amdgpu_waves_per_eu(4))) void d
 template <class T, int L, int P, bool GRAD>
 __global__ __launch_bounds__(256) void distill_group_kernel(DistillArgs a, int stride) {
     extern __shared__ int4 entries[];
-    __shared__ float s_part[4][3];
-    __shared__ int s_live[4];
     constexpr int R = 256 / L, N = T::vec;
+    __shared__ double s_linear[2][R], s_factor[2][R];
+    __shared__ int s_rows[R], s_live[4];
     const int slot = threadIdx.x / L, lane = threadIdx.x & (L - 1), r = blockIdx.x * R + slot, V = a.rows.V, K = a.K;
     const int full = V / N, rest = V - full * N;                // whole 16-byte pieces, and words behind them
     int *index = (int *)entries + slot * stride;                // [R][stride] each
@@ -539,7 +540,7 @@ __global__ __launch_bounds__(256) void distill_group_kernel(DistillArgs a, int s
 #pragma unroll
         for (int e = 0; e < N; ++e) zmax = fmaxf(zmax, element<T>(x[i], e));
     auto larger = [](float u, float v) { return fmaxf(u, v); };
-    auto plus = [](float u, float v) { return u + v; };
+    auto plus = [](double u, double v) { return u + v; };
     zmax = group_reduce<L>(zmax, larger);
     tmax = group_reduce<L>(tmax, larger);
 
@@ -562,29 +563,32 @@ __global__ __launch_bounds__(256) void distill_group_kernel(DistillArgs a, int s
             for (int e = 0; e < N; ++e) second[e] = __builtin_amdgcn_exp2f((z[e] - zmax) * kLog2e);
         }
     };
-    float s0 = 0.f, s1 = 0.f, A = 0.f, B = 0.f;
+    // in 64 bits: where the student nearly agrees with a teacher that names all words, little is left of these sums, and their
+    // roundings would be most of its error
+    double sum0 = 0.0, sum1 = 0.0, sumA = 0.0, sumB = 0.0;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
         float z[N], first[N], second[N];
         widen(x[i], z);
         exponentials(z, first, second);
 #pragma unroll
-        for (int e = 0; e < N; ++e) s0 += first[e];
+        for (int e = 0; e < N; ++e) sum0 += (double)first[e];
         if (two) {
 #pragma unroll
-            for (int e = 0; e < N; ++e) s1 += second[e];
+            for (int e = 0; e < N; ++e) sum1 += (double)second[e];
         }
     }
     for (int k = lane; k < K; k += L) {
-        const float t = share[k], d = (t - tmax) * a.inv_tau;
-        const float e = index[k] >= 0 && t != -INFINITY ? __builtin_amdgcn_exp2f(d * kLog2e) : 0.f;
-        if (e != 0.f) { A += e; B += e * (d - (words[k] - zmax) * a.inv_tau); }
+        const float t = share[k], d = t - tmax;
+        const float e = index[k] >= 0 && t != -INFINITY ? __builtin_amdgcn_exp2f(d * a0) : 0.f;
+        if (e != 0.f) { sumA += (double)e; sumB += (double)e * (double)(d - (words[k] - zmax)); }
         share[k] = e;
     }
-    s0 = group_reduce<L>(s0, plus);
-    s1 = two ? group_reduce<L>(s1, plus) : s0;
-    A = group_reduce<L>(A, plus);
-    B = group_reduce<L>(B, plus);
+    sum0 = group_reduce<L>(sum0, plus);
+    sum1 = two ? group_reduce<L>(sum1, plus) : sum0;
+    sumA = group_reduce<L>(sumA, plus);
+    sumB = group_reduce<L>(sumB, plus);
+    const float s0 = (float)sum0, s1 = (float)sum1, A = (float)sumA;
     if constexpr (GRAD) {
         int n = 0;
         if (!a.sum) n = a.live ? a.live[threadIdx.x & 63] : count_live(a, threadIdx.x, 256);
@@ -653,29 +657,45 @@ __global__ __launch_bounds__(256) void distill_group_kernel(DistillArgs a, int s
             if (lane == 0 && label >= 0 && named_label == 0.f) store1<T>(out, label, density(zy) - hard);
         }
     }
-    float part[3] = {0.f, 0.f, 0.f};
-    if (live && lane == 0) {
-        part[0] = hard_on ? logf(s1) - (zy - zmax) : 0.f;
-        part[1] = soft_on && A != 0.f ? B / A - logf(A) + logf(s0) : 0.f;
-        part[2] = 1.f;
-    }
-    wave_sum_n(part);
-    if ((threadIdx.x & 63) == 0) {
-#pragma unroll
-        for (int k = 0; k < 3; ++k) s_part[threadIdx.x >> 6][k] = part[k];
+    // the rows' losses are  linear + log(factor)  each; one logarithm takes the product of a workgroup's factors (each within
+    // 2^-8 .. 2^10, 64 of them at most)
+    if (lane == 0) {
+        const bool soft = live && soft_on && A != 0.f, hard = live && hard_on;
+        const double inverse = 1.0 / (soft ? sumA : 1.0);
+        s_linear[0][slot] = hard ? -(double)(zy - zmax) : 0.0;
+        s_factor[0][slot] = hard ? sum1 : 1.0;
+        s_linear[1][slot] = soft ? sumB * inverse * (a0 * 0.6931471805599453) : 0.0;
+        s_factor[1][slot] = soft ? sum0 * inverse : 1.0;
+        s_rows[slot] = live ? 1 : 0;
     }
     __syncthreads();
-    if (threadIdx.x < 3)
-        a.part[3 * (int64_t)blockIdx.x + threadIdx.x] = (double)s_part[0][threadIdx.x] + (double)s_part[1][threadIdx.x] +
-                                                        (double)s_part[2][threadIdx.x] + (double)s_part[3][threadIdx.x];
+    if (threadIdx.x >= 64) return;
+    const int i = threadIdx.x;
+    double linear[2], factor[2];
+    int rows = i < R ? s_rows[i] : 0;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) { linear[k] = i < R ? s_linear[k][i] : 0.0; factor[k] = i < R ? s_factor[k][i] : 1.0; }
+    auto over_rows = [](auto v, auto op) {
+        v = group_reduce<16>(v, op);
+#pragma unroll
+        for (int d = 16; d < R; d <<= 1) v = op(v, __shfl_xor(v, d));
+        return v;
+    };
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        linear[k] = over_rows(linear[k], plus);
+        factor[k] = over_rows(factor[k], [](double u, double v) { return u * v; });
+    }
+    rows = over_rows(rows, [](int u, int v) { return u + v; });
+    if (i < 3) a.part[3 * (int64_t)blockIdx.x + i] = i == 2 ? (double)rows : (i ? linear[1] : linear[0]) + log(i ? factor[1] : factor[0]);
 }
 
 // Rows of up to 8 pieces for each of 16 lanes go to groups of lanes: what a row costs whatever its length (reductions, the
 // teacher's entries, quotients: about 400 instructions of a wave) is then shared by 4 to 16 rows, where a workgroup of one wave
-// per row spends it on each.  262144 rows, loss and gradient / loss alone, against a wave per row: 100 words of float 89 / 47 for
-// 275 / 134 us, 200: 134 / 67 for 296 / 146, 500: 280 / 125 for 379 / 182; of bfloat16 120: 88 / 48 for 300 / 174, 500: 191 / 80
-// for 362 / 233; 32768 rows of 1000: 56 / 24 for 62 / 35.  (A word per lane: 9 words 31 / 16 for 55 / 37, 40 words 72 / 39 for
-// 175 / 134.)  Issue binds them up to some 200 words, the bytes beyond (500 words of float: 3.7 TB/s).
+// per row spends it on each.  262144 rows, loss and gradient / loss alone, against a wave per row: 100 words of float 94 / 53 for
+// 275 / 134 us, 200: 133 / 72 for 296 / 146, 500: 282 / 129 for 379 / 182; of bfloat16 120: 94 / 55 for 300 / 174, 500: 198 / 90
+// for 362 / 233; 32768 rows of 1000: 58 / 27 for 62 / 35.  (Against a word per lane: 9 words 32 / 17 for 55 / 37, 40 words 77 / 45
+// for 175 / 134.  Sums in 32 bits would be 3 to 10 % faster, a logarithm per row up to a third slower.)  Issue binds them up to some 200 words, the bytes beyond (500 words of float: 3.7 TB/s).
 constexpr int kGroupPieces = 8, kGroupLds = 48 * 1024;
 struct Group { int L, P, stride; };
 bool grouped(const gscan_rows &rows) { return cdiv(rows.V, rows.type == GSCAN_F32 ? 4 : 8) <= 16 * kGroupPieces; }

@@ -190,11 +190,12 @@ __device__ __forceinline__ V wave_reduce(V v, Op op) {
 // The same over groups of L = 4, 8 or 16 lanes, on the DPP datapath.  All lanes must be active.
 template <int CTRL, typename V>
 __device__ __forceinline__ V dpp_word(V v) {
-    static_assert(sizeof(V) == 4, "a word");
-    int w;
-    __builtin_memcpy(&w, &v, 4);
-    w = __builtin_amdgcn_update_dpp(0, w, CTRL, 0xf, 0xf, false);
-    __builtin_memcpy(&v, &w, 4);
+    static_assert(sizeof(V) == 4 || sizeof(V) == 8, "one word or two");
+    int w[sizeof(V) / 4];
+    __builtin_memcpy(w, &v, sizeof(V));
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(V) / 4; ++i) w[i] = __builtin_amdgcn_update_dpp(0, w[i], CTRL, 0xf, 0xf, false);
+    __builtin_memcpy(&v, w, sizeof(V));
     return v;
 }
 template <int L, typename V, class Op>

@@ -667,8 +667,7 @@ __global__ __launch_bounds__(256) void top_group_kernel(TopArgs a, int rows) {
             for (int e = i * N; e < i * N + N; ++e) s += z[e] == z[e] ? __builtin_amdgcn_exp2f((z[e] - m) * kLog2e) : 0.f;
             sum += s;
         }
-#pragma unroll
-        for (int k = 8; k; k >>= 1) sum += __shfl_xor(sum, k);
+        sum = group_reduce<16>(sum, [](double u, double v) { return u + v; });
         if (live && lane == 0) {
             if (a.parts) a.parts[r] = LsePart{sum, m, 0.f};
             else a.lse[r] = m == INFINITY ? INFINITY : (float)((double)m + log(sum));

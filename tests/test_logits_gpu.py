@@ -246,6 +246,19 @@ def test_distillation_of_short_rows(ops, dtype, lead, V, K):
         check_loss(ops.distillation_loss(zd, idd, td, yd, **kw), want, rows * weight * (2 + math.log(V)))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [2, 4, 31, 60, 250])
+@pytest.mark.parametrize("temperature", [1.0, 2.0, 3.5])
+def test_a_student_that_agrees_has_no_divergence(ops, dtype, V, temperature):
+    """A teacher that names every word and a student with the same logits: equal exponentials, summed in 64 bits in two orders —
+    2 V steps of 2^-53 at most, times temperature^2."""
+    z = (torch.randn(5, V, generator=gen(V, 71)) * 2).to(dtype)
+    index = torch.stack([torch.randperm(V, generator=gen(V, r)) for r in range(5)]).int()
+    teacher = z.gather(1, index.long())
+    loss = ops.distillation_loss(z.cuda(), index.cuda(), teacher.cuda(), temperature=temperature)
+    assert abs(loss.item()) <= 2 * (V + 4) * 2.0 ** -53 * temperature ** 2
+
+
 @pytest.mark.parametrize("n,V", [(8193, 1030), (131200, 70)])
 def test_sums_of_many_rows(ops, n, V):
     """More workgroups than one launch adds up; the mean is counted by a launch of its own."""
