@@ -6,8 +6,9 @@
 // words are >= the K-th largest of these maxima, so it bounds the K-th largest word from below.  LDS holds 16 bits of the
 // maximum of every 16-byte piece: the few pieces that reach the bound are read again, their words >= the bound (little more
 // than K unless many are equal) are ranked by counting.  Without the pieces' maxima a thread's whole share of the row would be
-// read again for every thread above the bound, a 128-byte line for every 16 bytes: 68 against 57 us for 4088 rows of 32000
-// bfloat16 words, K = 64.
+// read again for every thread above the bound, a 128-byte line for every 16 bytes: 73 against 61 us for 4088 rows of 32000
+// bfloat16 words, K = 64 (4.3 TB/s; a copy of 1 GiB reads and writes 5.05).  Few rows are split over workgroups and joined: one
+// row of 131072 float words takes 8 + 7.5 us, latencies (a dozen dependent steps each) and no bytes.
 // Exact for any input: where the words >= the bound do not fit the list, words above it and, in index order, words equal to
 // it are taken apart, and if even the words above it do not fit (a row laid out against the threads), a radix selection over
 // the row finds the K-th key.
