@@ -178,16 +178,19 @@ class _DistillationLoss(torch.autograd.Function):
     def forward(ctx, logits, indices, teacher, labels, options):
         device, logits, rows, terms, kept = _distillation(logits, indices, teacher, labels, *options)
         ctx.save_for_backward(logits, *kept)
-        ctx.options = options
+        ctx.options, ctx.call = options, (device, rows, terms, logits.stride())
         return _launch_distillation(device, logits, rows, terms, None, None)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         logits, indices, teacher, labels = ctx.saved_tensors
-        device, logits, rows, terms, _ = _distillation(logits, indices, teacher, labels, *ctx.options)
+        device, rows, terms, stride = ctx.call
+        if not (logits.data_ptr() == rows.data and logits.stride() == stride and indices.data_ptr() == terms.indices and teacher.data_ptr() == terms.teacher
+                and (labels is None or labels.data_ptr() == terms.labels)):       # hooks on saved tensors may have moved them
+            device, logits, rows, terms, _kept = _distillation(logits, indices, teacher, labels, *ctx.options)
         grad = _gradient(logits)
-        _launch_distillation(device, logits, rows, terms, g.to(torch.float32).contiguous(), grad, want_loss=False)
+        _launch_distillation(device, logits, rows, terms, g, grad, want_loss=False)
         return grad, None, None, None, None
 
 

@@ -405,6 +405,31 @@ def test_distillation_gradient_against_differences(ops, V):
             assert abs(slope - grad[0, row, word].item()) < 1.5 * h * h / 6 + 2 * 40 * 2.0 ** -23 / (2 * h), (word, row)
 
 
+@pytest.mark.parametrize("V", [9, 300, 5000])
+def test_backward_with_tensors_saved_elsewhere(ops, V):
+    """Hooks on saved tensors (kept on the host, copied back for the backward pass, with other strides and addresses) change
+    nothing; logits changed in place between the passes raise."""
+    z, index, teacher, labels = student((3, 4), V, 5, torch.float32, 77)
+    z, index, teacher, labels = z.cuda(), index.cuda(), teacher.cuda(), labels.cuda()
+    kw = dict(hard_weight=0.5, temperature=2.0)
+    want = ops.distillation_loss_and_gradient(z, index, teacher, labels, **kw)[1]
+    for view in (z, torch.stack([z, z], 1)[:, 0]):
+        leaf = view.detach().requires_grad_()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda()):
+            loss = ops.distillation_loss(leaf, index, teacher, labels, **kw)
+        assert torch.equal(torch.autograd.grad(loss, leaf)[0], want)
+        leaf = view.detach().requires_grad_()
+        loss = ops.distillation_loss(leaf, index, teacher, labels, **kw)
+        assert torch.equal(torch.autograd.grad(loss, leaf, retain_graph=True)[0], want)
+        assert torch.equal(torch.autograd.grad(loss, leaf)[0], want)
+    leaf = (z * 1.0).requires_grad_()
+    moved = leaf * 1.0
+    loss = ops.distillation_loss(moved, index, teacher, labels, **kw)
+    moved.detach().add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # beam search
 # ---------------------------------------------------------------------------------------------------------------------
