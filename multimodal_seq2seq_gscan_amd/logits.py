@@ -14,6 +14,7 @@ import functools
 from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -209,11 +210,13 @@ def distillation_loss(logits: torch.Tensor, teacher_indices: torch.Tensor, teach
     labels [...] int64: rows whose label is `ignore_index` or not a word are not live — no loss, a gradient of exactly 0,
     nothing of them is read; without labels every row is live.  `shift_labels`: labels are whole sequences and a row is
     scored against the next one, the last against 0, as `Model.get_loss` does (seq2seq/model.py:108-115).
-    reduction "mean" (0 when no row is live) or "sum".  A differentiable float32 scalar; the gradient goes to `logits` only.
+    reduction "mean" (0 when no row is live) or "sum".  A differentiable float32 scalar; the gradient goes to `logits` only
+    (backward only: logits with a forward-mode tangent raise).
     Into a graph, capture the backward pass of a loss that was captured too, with no eager loss of the same parameters alive
     (autograd adds up a parameter's gradient on the stream that it was first used on)."""
     options = (temperature, soft_weight, hard_weight, ignore_index, shift_labels, reduction)
-    if torch.is_grad_enabled() and logits.requires_grad:
+    # a tangent too is autograd's to deal with: it raises, this function having no forward-mode derivative
+    if (torch.is_grad_enabled() and logits.requires_grad) or forward_ad.unpack_dual(logits).tangent is not None:
         return _DistillationLoss.apply(logits, teacher_indices, teacher_logits, labels, options)
     device, logits, rows, terms, _kept = _distillation(logits, teacher_indices, teacher_logits, labels, *options)
     return _launch_distillation(device, logits, rows, terms, None, None)
