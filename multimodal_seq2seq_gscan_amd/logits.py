@@ -378,7 +378,10 @@ def beam_reorder(parents: torch.Tensor, states: Union[torch.Tensor, Sequence[tor
             raise ValueError(f"out[{i}] must be {tuple(s.shape)} of {s.dtype}, got {tuple(d.shape)} of {d.dtype}")
         if s.numel() == 0:
             continue
+        s = s.resolve_conj().resolve_neg()         # bytes are moved: a conjugation that only the view knows of would be lost
         if out is not None:
+            if d.is_conj() or d.is_neg():
+                raise ValueError(f"out[{i}] is a lazily conjugated or negated view")
             if any(_overlap(d, other) for other in (parents, *sources)):
                 raise ValueError(f"out[{i}] shares memory with a state or with the parents")
             if _overlaps_itself(d):
