@@ -58,6 +58,7 @@ def _rows(logits: torch.Tensor) -> Tuple[torch.Tensor, _lib.Rows]:
     """The rows of `logits` [..., V] as the library takes them: the last leading dimension is `inner`, those before it one
     `outer` dimension.  Copies only where no pair of strides describes them (or the words of a row are not adjacent)."""
     kind = _float_type(logits, "logits")
+    logits = logits.resolve_neg()        # the library reads memory: a sign that only a view knows of would be lost
     shape, stride = logits.shape, logits.stride()
     n = len(shape)
     if n == 0 or shape[-1] == 0:
@@ -145,7 +146,7 @@ def _distillation(logits, teacher_indices, teacher_logits, labels, temperature, 
         if labels.shape != lead:
             raise ValueError(f"labels must be {tuple(lead)}, got {tuple(labels.shape)}")
         labels = labels.contiguous()
-    indices, teacher = teacher_indices.contiguous(), teacher_logits.contiguous()
+    indices, teacher = teacher_indices.contiguous(), teacher_logits.resolve_neg().contiguous()
     terms = _lib.Distillation(indices.data_ptr(), teacher.data_ptr(), _lib.ptr(labels), int(ignore_index),
                               _INDEX_BITS[indices.dtype], kind, K, int(bool(shift_labels)), temperature, soft_weight, hard_weight,
                               int(reduction == "sum"))
@@ -191,7 +192,7 @@ class _DistillationLoss(torch.autograd.Function):
                 and (labels is None or labels.data_ptr() == terms.labels)):       # hooks on saved tensors may have moved them
             device, logits, rows, terms, _kept = _distillation(logits, indices, teacher, labels, *ctx.options)
         grad = _gradient(logits)
-        _launch_distillation(device, logits, rows, terms, g, grad, want_loss=False)
+        _launch_distillation(device, logits, rows, terms, g.resolve_neg(), grad, want_loss=False)
         return grad, None, None, None, None
 
 
@@ -242,6 +243,8 @@ def _check_gradient_out(out: torch.Tensor, logits: torch.Tensor, others: Sequenc
     _require("logits out", logits, out)
     if out.shape != logits.shape or out.dtype != logits.dtype or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {tuple(logits.shape)} tensor of {logits.dtype}")
+    if out.is_neg():
+        raise ValueError("out is a lazily negated view")
     if any(t is not None and _overlap(out, t) for t in (logits, *others)):
         raise ValueError("out shares memory with the logits, the teacher's entries or the labels")
 
@@ -294,7 +297,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
     if not (0 <= int(eos_idx) < V and 0 <= int(pad_idx) < V):
         raise ValueError(f"eos_idx {eos_idx} or pad_idx {pad_idx} is not one of the {V} words")
     where = logits.device
-    scores, finished = scores.contiguous(), finished.contiguous()
+    scores, finished = scores.resolve_neg().contiguous(), finished.contiguous()
     new_scores = torch.empty(B, W, dtype=torch.float32, device=where)
     parents = torch.empty(B, W, dtype=torch.int32, device=where)
     words = torch.empty(B, W, dtype=torch.int64, device=where)

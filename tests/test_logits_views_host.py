@@ -75,3 +75,48 @@ def test_outputs_that_are_written_through_a_conjugation_are_refused(on_host):
         with pytest.raises(ValueError, match="conjugat"):
             ops.beam_reorder(parents, torch.zeros(6, 5, dtype=out.dtype), out=out)
     assert not on_host
+
+
+def floats_at(address, like):
+    import ctypes as C
+    return torch.tensor(list((C.c_float * like.numel()).from_address(address))).view(like.shape)
+
+
+def test_lazily_negated_logits_scores_and_gradients_are_read_by_value(on_host, monkeypatch):
+    """Everything that the library reads as floats: what lies at the addresses that it is given."""
+    seen = []
+
+    def call(name, device, rows, *args):
+        rows = rows._obj
+        took = [floats_at(rows.data, torch.empty(rows.outer, rows.inner, rows.V))]
+        if name == "gscan_distillation_loss":
+            terms, upstream = args[0]._obj, args[1]
+            took.append(floats_at(terms.teacher, torch.empty(rows.outer, rows.inner, terms.K)))
+            if upstream:
+                took.append(floats_at(upstream, torch.empty(())))
+        if name == "gscan_beam_select":
+            took.append(floats_at(args[0], torch.empty(rows.outer, rows.inner)))
+        seen.append(took)
+    monkeypatch.setattr(ops, "_call", call)
+    # adjacent words: the imaginary parts of complex numbers lie two floats apart
+    logits, teacher, scores = (torch._neg_view(torch.randn(*shape)) for shape in ((2, 3, 10), (2, 3, 4), (2, 3)))
+    index = torch.zeros(2, 3, 4, dtype=torch.int32)
+    ops.top_logits(logits, 2)
+    ops.distillation_loss(logits, index, teacher)
+    ops.distillation_loss_and_gradient(logits, index, teacher)
+    ops.beam_select(logits, scores, torch.zeros(2, 3, dtype=torch.bool), eos_idx=2, pad_idx=0)
+    assert len(seen) == 4
+    for took, want in zip(seen, ([logits], [logits, teacher], [logits, teacher], [logits, scores])):
+        assert all(torch.equal(a, b) for a, b in zip(took, want)) and len(took) == len(want)
+    # a gradient that arrives negated: that of the imaginary part of a conjugated number
+    leaf = torch.randn(2, 3, 10, requires_grad=True)
+    loss = ops.distillation_loss(leaf, index, teacher)
+    torch.complex(torch.zeros(()), loss).conj().backward(torch.complex(torch.tensor(0.0), torch.tensor(3.0)))
+    assert seen[-1][2].item() == -3.0
+    # and from the operator's own entry to a number of other strides
+    x = conjugated(4, 2, 3, 10)[1]
+    ops.top_logits(x, 2)
+    assert torch.equal(seen[-1][0], x)
+    grad = torch.zeros(2, 3, 10)
+    with pytest.raises(ValueError, match="negated"):
+        ops.distillation_loss_and_gradient(logits, index, teacher, out=torch._neg_view(grad))
