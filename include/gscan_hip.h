@@ -377,11 +377,12 @@ int gscan_distillation_loss(const gscan_rows *rows, const gscan_distillation *te
                             float *loss, float *stats, void *workspace, size_t workspace_bytes, void *stream);
 
 /* One step of beam search over `outer` batch rows of `inner` beams (at most GSCAN_MAX_BEAMS): the `inner` best candidates by
- * scores[b, w] + log_softmax(logits[b, w])[v], ties to the lowest w * V + v, in order.  A beam with finished[b, w] != 0 has
+ * scores[b, w] + log_softmax(logits[b, w])[v] (compared in 64 bits), in order; of equal scores the lowest beam's is first, of
+ * one beam's the largest logit, of equal ones the lowest word.  A beam with finished[b, w] != 0 has
  * one candidate, itself with its score unchanged and the word `pad`; its logits are not read.  A beam with the score -inf
  * (a search's first step: every beam but one) is not read either and fills places that nothing else takes, as do candidates
- * of score -inf (word barred by -inf, NaN), in order of w * V + v.  Logits of +inf have no log_softmax: such a beam's
- * candidates count as -inf.  Outputs [outer, inner]: score, parent beam, word, finished (the parent was, or word == eos). */
+ * of score -inf (word barred by -inf, NaN), in order of w * V + v.  A score of NaN counts as -inf, as do the candidates of a
+ * beam with a logit of +inf, which has no log_softmax.  Outputs [outer, inner]: score, parent beam, word, finished (the parent was, or word == eos). */
 size_t gscan_beam_select_workspace_bytes(const gscan_rows *rows);
 int gscan_beam_select(const gscan_rows *rows, const float *scores, const uint8_t *finished, int eos, int pad, float *scores_out,
                       int32_t *parents, int64_t *tokens, uint8_t *finished_out, void *workspace, size_t workspace_bytes,

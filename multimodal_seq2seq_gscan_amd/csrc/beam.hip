@@ -1,10 +1,13 @@
 // One step of beam search: the W best continuations of a batch row's W beams, and the beams' states put in the new order.
 //
 // A candidate (w, v) has the score  score_w + z[w, v] - lse(z[w, :]);  a finished beam has one candidate, itself with its
-// score as it is and a padding word; the order is score descending, then w V + v ascending.  Within a beam that is the order of
-// the words, so the W best of every beam (top_logits.hip, one pass over the logits, with the beam's softmax sum) hold the W best
+// score as it is and a padding word.  The order is score descending, then w ascending, then, within a beam, logit descending (which
+// decides where scores that lie far out round to the same number) and v ascending.  Within a beam that is the order of the
+// logits alone, so the W best of every beam (top_logits.hip, one pass over the logits, with the beam's softmax sum) hold the W best
 // of all: W sorted lists (W times the chunks of a row) that one wave merges by W rounds over the lists' heads.  Scores are
-// compared in 64 bits: candidates of different beams come closer to each other than 32 bits of a sum tell apart.
+// compared in 64 bits: candidates of different beams come closer to each other than 32 bits of a sum tell apart.  A beam whose
+// candidates all score -inf whatever their logits (its own score is -inf or NaN, or its logits have no log-softmax) has them in
+// the order of v.
 #include "logits.h"
 
 namespace gscan {
@@ -38,6 +41,9 @@ __device__ __forceinline__ uint64_t score_key(double score, double z, double lse
     return order_key64(s == s ? s : -INFINITY);
 }
 
+// whether the logits of a beam order its candidates (else all of them score -inf)
+__device__ __forceinline__ bool by_logit(float score, double lse) { return score > -INFINITY && fabs(lse) < INFINITY; }
+
 // Joins the lists of a batch row's beams: W rounds of one wave, each a reduction and one lane's two LDS reads, behind the lists'
 // way into LDS.  Latencies bind it: 5.8 us for one row's 16 lists of 4, 10.5 for 32 rows' 16 lists of 8.
 __global__ __launch_bounds__(256) void beam_join_kernel(BeamArgs a) {
@@ -66,7 +72,7 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamArgs a) {
         uint32_t v = 0;
         if (s_done[w]) {
             if (c == 0 && k == 0) { key = score_key((double)score, 0.0, 0.0); v = (uint32_t)a.pad; }
-        } else if (score == -INFINITY) {
+        } else if (!by_logit(score, s_lse[w])) {
             if (c == 0) { key = order_key64(-INFINITY); v = (uint32_t)k; }
         } else {
             const uint64_t x = i == tid ? early : keys[i];
@@ -81,18 +87,25 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamArgs a) {
     uint64_t best = 0;
     uint32_t flat = ~0u;
     int from = -1;
+    // what decides between the heads of two lists of one beam whose scores are equal: the larger comes first
+    auto within = [&](int l, int w) {
+        const int i = l * a.K + s_head[l];
+        return s_done[w] || !by_logit(s_score[w], s_lse[w]) ? pair_key(0u, (int)(s_flat[i] - (uint32_t)w * (uint32_t)a.rows.V)) : keys[i];
+    };
+    auto before = [&](int l, int m) {
+        const int w = l / a.splits, o = m / a.splits;
+        return w != o ? w < o : within(l, w) > within(m, o);
+    };
     auto refresh = [&]() {
         best = 0; flat = ~0u; from = -1;
         for (int l = tid; l < lists; l += 64) {
             const int h = s_head[l];
             if (h >= a.K) continue;
             const uint64_t k = s_key[l * a.K + h];
-            const uint32_t f = s_flat[l * a.K + h];
-            if (k > best || (k == best && k && f < flat)) { best = k; flat = f; from = l; }
+            if (k > best || (k == best && k && before(l, from))) { best = k; flat = s_flat[l * a.K + h]; from = l; }
         }
     };
     auto largest = [](uint32_t x, uint32_t y) { return max(x, y); };
-    auto smallest = [](uint32_t x, uint32_t y) { return min(x, y); };
     refresh();
     for (int place = 0; place < a.W; ++place) {
         // the high words settle it unless two scores come within 2^-20 of each other
@@ -100,11 +113,15 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamArgs a) {
         bool in = (uint32_t)(best >> 32) == high;
         if (__popcll(__ballot(in)) > 1) {
             const uint32_t low = wave_reduce(in ? (uint32_t)best : 0u, largest);
-            in = in && (uint32_t)best == low;
-            const uint32_t first = wave_reduce(in ? flat : ~0u, smallest);
-            in = in && flat == first;
+            in = in && (uint32_t)best == low && from >= 0;
+            if (__popcll(__ballot(in)) > 1) {        // equal: the lowest beam, then (chunks of one row) as `within` says
+                const int w = in ? from / a.splits : kMaxBeams, lowest = wave_reduce(w, [](int x, int y) { return min(x, y); });
+                in = in && w == lowest;
+                const double x = in ? pair_double(within(from, w)) : -1.0, first = wave_reduce(x, [](double u, double v) { return fmax(u, v); });
+                in = in && x == first;
+            }
         }
-        if (in && from >= 0) {                       // one lane: candidates differ in `flat`
+        if (in && from >= 0) {                       // one lane: heads of one beam differ in their words
             s_head[from] += 1;
             put_beam(a, b, place, best, flat);
             refresh();
@@ -118,6 +135,7 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamArgs a) {
 template <class T, int L>
 __global__ __launch_bounds__(256) void beam_small_kernel(BeamArgs a) {
     __shared__ uint64_t s_key[256];
+    __shared__ uint32_t s_word[256];                         // what decides between words of one beam of equal scores
     const int W = a.W, V = a.rows.V, per = 256 / L / W;      // batch rows per workgroup
     const int slot = threadIdx.x / L, v = threadIdx.x & (L - 1), mine = slot / W, w = slot - mine * W;
     const int b = blockIdx.x * per + mine;
@@ -134,19 +152,30 @@ __global__ __launch_bounds__(256) void beam_small_kernel(BeamArgs a) {
 #pragma unroll
     for (int d = L / 2; d; d >>= 1) s += __shfl_xor(s, d, L);
     uint64_t key = 0;
+    uint32_t order = 0;
     if (word) {
         if (done) key = v == a.pad ? score_key((double)score, 0.0, 0.0) : 0ull;
         else if (dead) key = order_key64(-INFINITY);
-        else key = score_key((double)score, (double)z, (double)m + log(s));
+        else {
+            const double lse = (double)m + log(s);
+            key = score_key((double)score, (double)z, lse);
+            if (by_logit(score, lse)) order = order_key(z);
+        }
     }
     s_key[threadIdx.x] = key;
+    s_word[threadIdx.x] = order;
     __syncthreads();
     if (!key) return;
     const int first = mine * W * L, i = threadIdx.x - first;
     int place = 0;
     for (int j = 0; j < W * L; ++j) {
         const uint64_t o = s_key[first + j];
-        place += o > key || (o == key && j < i) ? 1 : 0;
+        bool ahead = o > key;
+        if (o == key) {
+            const uint32_t other = j / L == i / L ? s_word[first + j] : order;
+            ahead = other > order || (other == order && j < i);
+        }
+        place += ahead ? 1 : 0;
     }
     if (place < W) put_beam(a, b, place, key, (uint32_t)w * (uint32_t)V + (uint32_t)v);
 }

@@ -279,10 +279,12 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
 
     logits [B, W, V] of the next word, scores [B, W] float32 (the beams' log-probabilities so far), finished [B, W] bool.
     A candidate's score is `scores[b, w] + log_softmax(logits[b, w])[v]`; a finished beam has one candidate, itself with its
-    score as it is and the word `pad_idx`, and its logits are not read.  Returns, best first (ties to the lowest w * V + v):
+    score as it is and the word `pad_idx`, and its logits are not read.  Returns, best first (scores are
+    compared in 64 bits; of equal ones the lowest beam's comes first, of one beam's the largest logit, then the lowest word):
     (scores [B, W], parents [B, W] int32, words [B, W] int64, finished [B, W] bool: the parent was, or the word is `eos_idx`).
     Start a search with scores of 0 for one beam and -inf for the others: beams of -inf fill only places that nothing else
-    takes.  W <= 64, V <= 2^24; a word barred with -inf (or NaN) has the score -inf."""
+    takes.  W <= 64, V <= 2^24; a word barred with -inf (or NaN) has the score -inf, as
+    have all words of a beam whose score is NaN or one of whose logits is +inf."""
     device = _require("logits scores finished", logits, scores, finished)
     if logits.dim() != 3:
         raise ValueError(f"logits must be [B, W, V], got {tuple(logits.shape)}")
