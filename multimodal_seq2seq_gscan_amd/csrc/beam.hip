@@ -153,13 +153,20 @@ __global__ __launch_bounds__(256) void beam_small_kernel(BeamArgs a) {
     for (int d = L / 2; d; d >>= 1) s += __shfl_xor(s, d, L);
     uint64_t key = 0;
     uint32_t order = 0;
+    bool close = false;
     if (word) {
         if (done) key = v == a.pad ? score_key((double)score, 0.0, 0.0) : 0ull;
         else if (dead) key = order_key64(-INFINITY);
         else {
             const double lse = (double)m + log(s);
             key = score_key((double)score, (double)z, lse);
-            if (by_logit(score, lse)) order = order_key(z);
+            if (by_logit(score, lse)) {
+                // does the next float up or down score the same?  (nothing between them can, if it does not)
+                const uint32_t bits = __float_as_uint(z);
+                order = order_key(z);
+                close = score_key((double)score, (double)__uint_as_float(bits + 1), lse) == key ||
+                        score_key((double)score, (double)__uint_as_float(bits - 1), lse) == key;
+            }
         }
     }
     s_key[threadIdx.x] = key;
@@ -170,12 +177,11 @@ __global__ __launch_bounds__(256) void beam_small_kernel(BeamArgs a) {
     int place = 0;
     for (int j = 0; j < W * L; ++j) {
         const uint64_t o = s_key[first + j];
-        bool ahead = o > key;
-        if (o == key) {
-            const uint32_t other = j / L == i / L ? s_word[first + j] : order;
-            ahead = other > order || (other == order && j < i);
-        }
-        place += ahead ? 1 : 0;
+        place += o > key || (o == key && j < i) ? 1 : 0;
+    }
+    if (close) {                         // this beam's words of the same score: by logit (in the loop above: 9.7 us in place of 6)
+        for (int j = w * L; j < w * L + L; ++j)
+            if (s_key[first + j] == key) place += (s_word[first + j] > order ? 1 : 0) - (s_word[first + j] != order && j < i ? 1 : 0);
     }
     if (place < W) put_beam(a, b, place, key, (uint32_t)w * (uint32_t)V + (uint32_t)v);
 }

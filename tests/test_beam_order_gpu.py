@@ -8,7 +8,7 @@ from test_logits_gpu import NEG, TYPES, gen, ops  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
-SIZES = [(3, 4, 9), (2, 16, 9), (2, 20, 9), (1, 4, 64), (2, 4, 200), (1, 4, 1000), (2, 3, 9000), (1, 6, 40003)]
+SIZES = [(3, 4, 9), (2, 16, 9), (2, 8, 5), (3, 7, 30), (2, 20, 9), (1, 4, 64), (2, 4, 200), (1, 4, 1000), (2, 3, 9000), (1, 6, 40003)]
 
 
 def ordered(logits, scores, finished, eos, pad):
