@@ -739,7 +739,9 @@ template <class T, int TPB>
 int launch_rows(const TopArgs &a, int64_t grid, bool lse, hipStream_t stream) {
     const int pieces = cdiv(a.chunk, T::vec);
     if (pieces <= 4 * TPB) return launch_rows<T, TPB, 0>(a, grid, lse, stream);
-    if (TPB == 64 || pieces <= 16 * TPB) return launch_rows<T, TPB, 16 * TPB>(a, grid, lse, stream);      // a wave: 2048 words at most
+    if constexpr (TPB == 256 || T::vec == 4) {       // a wave's 2048 words at most: of 16 bits they are 4 pieces a lane
+        if (TPB == 64 || pieces <= 16 * TPB) return launch_rows<T, TPB, 16 * TPB>(a, grid, lse, stream);
+    }
     return launch_rows<T, 256, 32 * 256>(a, grid, lse, stream);
 }
 template <class T>
