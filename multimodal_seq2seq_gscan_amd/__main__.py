@@ -154,6 +154,8 @@ def main(flags):
         assert flags["input_vocab_path"] and flags["target_vocab_path"], "Please specify paths to vocabularies to save."
     if flags["test_batch_size"] > 1:
         raise NotImplementedError("Test batch size larger than 1 not implemented.")
+    from .predict import check_beam_size
+    check_beam_size(flags.get("beam_size", 1))
 
     if flags["mode"] == "train":
         from .config import model_kwargs

@@ -104,6 +104,13 @@ def greedy_decode_stepwise(model, commands: torch.Tensor, cmd_lengths, world: to
     return rows
 
 
+def check_beam_size(beam_size: int) -> int:
+    """The beam size as a whole number; 1 decodes greedily."""
+    if not 1 <= int(beam_size) <= _lib.MAX_BEAMS:
+        raise ValueError(f"beam_size must be 1 to {_lib.MAX_BEAMS}, got {beam_size}")
+    return int(beam_size)
+
+
 def beam_decode(model, commands: torch.Tensor, cmd_lengths, world: torch.Tensor, sos_idx: int, eos_idx: int,
                 max_decoding_steps: int, beam_size: int, pad_idx: int = 0, length_penalty: float = 0.0) -> dict:
     """Beam search (not in the reference) in the place of `greedy_decode`, with its limits: `beam_size` continuations of
@@ -114,9 +121,8 @@ def beam_decode(model, commands: torch.Tensor, cmd_lengths, world: torch.Tensor,
 
     The rows' commands and worlds are encoded once per beam, so that beams are rows to the decoder's step kernel; words,
     parents and attention rows stay on the device until the search has ended, and the host looks at it every eighth step."""
-    B, W, device = commands.shape[0], int(beam_size), commands.device
-    if not 1 <= W <= _lib.MAX_BEAMS:
-        raise ValueError(f"beam_size must be 1 to {_lib.MAX_BEAMS}, got {beam_size}")
+    W = check_beam_size(beam_size)
+    B, device = commands.shape[0], commands.device
     lengths = [int(v) for v in (cmd_lengths.tolist() if isinstance(cmd_lengths, torch.Tensor) else cmd_lengths)]
     per_beam = [n for n in lengths for _ in range(W)]
     encoded = model.encode_input(commands_input=commands.repeat_interleave(W, 0), commands_lengths=per_beam,
@@ -175,6 +181,7 @@ def predict(data_iterator: Iterator, model, max_decoding_steps: int, pad_idx: in
     size; one 8-tuple is yielded per example:
     (input_sequence [1,L], derivation_spec, situation_spec, output_sequence, target_sequence [1,T],
      attention_weights_commands, attention_weights_situations, auxiliary_accuracy_target)."""
+    beam_size = check_beam_size(beam_size)
     model.eval()
     start = time.time()
     count = 0

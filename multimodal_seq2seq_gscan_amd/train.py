@@ -654,8 +654,9 @@ def train_on_dataset(data_path: str, data_directory: str, generate_vocabularies:
     import numpy as np
     from .config import model_kwargs
     from .dataset import BatchStager, GroundedScanDataset
-    from .predict import evaluate_sums
+    from .predict import check_beam_size, evaluate_sums
 
+    check_beam_size(beam_size)                                  # not at the first evaluation
     torch.manual_seed(seed)                                     # train.py:27
     np.random.seed(seed)                                        # the same shuffle on every rank
     random.seed(seed)                                           # the same k-shot sample on every rank (dataset.load_examples)
