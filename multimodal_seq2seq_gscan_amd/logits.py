@@ -1,8 +1,7 @@
 """Operators over rows of logits, on libgscan_hip.so: the top K of every row, distillation from a teacher's top logits, the
 step of a beam search.
 
-The model facade builds on them (`Model.top_logits`, `Model.get_distillation_loss`, `train.TrainStep(teacher=...)`,
-`predict.beam_decode`); they take any vocabulary, in float32, bfloat16 or float16.  Logits are read where they are: `[..., V]`
+The framework builds on them (`Model.get_distillation_loss`, `train.TrainStep(teacher=...)`, `predict.beam_decode`); they take any vocabulary, in float32, bfloat16 or float16.  Logits are read where they are: `[..., V]`
 with adjacent words and any strides in front of them (a slice of a longer batch, an expanded dimension).  Every call runs on
 the current stream of its tensors' device, allocates what it returns and its workspace from torch's allocator, and neither
 synchronises nor keeps anything between calls, so it can be captured in a graph.  CPU tensors raise: there is no CPU path in
@@ -284,7 +283,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
     (scores [B, W], parents [B, W] int32, words [B, W] int64, finished [B, W] bool: the parent was, or the word is `eos_idx`).
     Start a search with scores of 0 for one beam and -inf for the others: beams of -inf fill only places that nothing else
     takes.  W <= 64, V <= 2^24; a word barred with -inf (or NaN) has the score -inf, as
-    have all words of a beam whose score is NaN or one of whose logits is +inf."""
+    have all words of a beam whose score is NaN or one of whose logits is +inf.  No gradient flows through it."""
     device = _require("logits scores finished", logits, scores, finished)
     if logits.dim() != 3:
         raise ValueError(f"logits must be [B, W, V], got {tuple(logits.shape)}")
@@ -359,7 +358,7 @@ def beam_reorder(parents: torch.Tensor, states: Union[torch.Tensor, Sequence[tor
     them, all moved in one launch (16 at a time).  `out`: where to write (of the states' shapes, any strides: a slice of a
     longer cache keeps what lies behind it), in memory whose span, from its first element to its last, meets neither a state's
     nor another `out`'s; otherwise new contiguous tensors are returned.
-    A parent outside [0, W) gives zeros."""
+    A parent outside [0, W) gives zeros.  No gradient flows through it."""
     single = isinstance(states, torch.Tensor)
     sources = [states] if single else list(states)
     if parents.dim() != 2 or parents.dtype != torch.int32:

@@ -429,7 +429,8 @@ class TrainStep:
             if teacher is model:
                 raise ValueError("a model cannot be its own teacher: one step is in flight per model")
             if teacher._hyper["V"] != model._hyper["V"] or teacher._hyper["Vi"] != model._hyper["Vi"] or teacher._hyper["C"] != model._hyper["C"]:
-                raise ValueError("teacher and student must share their vocabularies and the world's channels")
+                raise ValueError("teacher and student must have vocabularies of the same sizes (a checkpoint does not hold their words: "
+                                 "that they are the same is the caller's to see to) and the same channels of the world")
             if not 0.0 <= float(distill_weight) <= 1.0:
                 raise ValueError(f"distill_weight must be 0 to 1, got {distill_weight}")
             if int(distill_top_k) < 1:
