@@ -1,11 +1,11 @@
 """Operators over rows of logits, on libgscan_hip.so: the top K of every row, distillation from a teacher's top logits, the
 step of a beam search.
 
-The framework builds on them (`Model.get_distillation_loss`, `train.TrainStep(teacher=...)`, `predict.beam_decode`); they take any vocabulary, in float32, bfloat16 or float16.  Logits are read where they are: `[..., V]`
-with adjacent words and any strides in front of them (a slice of a longer batch, an expanded dimension).  Every call runs on
-the current stream of its tensors' device, allocates what it returns and its workspace from torch's allocator, and neither
-synchronises nor keeps anything between calls, so it can be captured in a graph.  CPU tensors raise: there is no CPU path in
-this package."""
+The framework builds on them (`Model.get_distillation_loss`, `train.TrainStep(teacher=...)`, `predict.beam_decode`); they take
+any vocabulary, in float32, bfloat16 or float16.  Logits are read where they are: `[..., V]` with adjacent words and any strides
+in front of them (a slice of a longer batch, an expanded dimension).  Every call runs on the current stream of its tensors'
+device, allocates what it returns and its workspace from torch's allocator, and neither synchronises nor keeps anything between
+calls, so it can be captured in a graph.  CPU tensors raise: there is no CPU path in this package."""
 from __future__ import annotations
 
 import ctypes as C
@@ -57,7 +57,8 @@ def _rows(logits: torch.Tensor) -> Tuple[torch.Tensor, _lib.Rows]:
     """The rows of `logits` [..., V] as the library takes them: the last leading dimension is `inner`, those before it one
     `outer` dimension.  Copies only where no pair of strides describes them (or the words of a row are not adjacent)."""
     kind = _float_type(logits, "logits")
-    logits = logits.resolve_neg()        # the library reads memory: a sign that only a view knows of would be lost
+    if logits.is_neg():          # the library reads memory: a sign that only the view knows of would be lost
+        logits = logits.resolve_neg()
     shape, stride = logits.shape, logits.stride()
     n = len(shape)
     if n == 0 or shape[-1] == 0:
@@ -145,7 +146,9 @@ def _distillation(logits, teacher_indices, teacher_logits, labels, temperature, 
         if labels.shape != lead:
             raise ValueError(f"labels must be {tuple(lead)}, got {tuple(labels.shape)}")
         labels = labels.contiguous()
-    indices, teacher = teacher_indices.contiguous(), teacher_logits.resolve_neg().contiguous()
+    indices, teacher = teacher_indices.contiguous(), teacher_logits.contiguous()
+    if teacher.is_neg():
+        teacher = teacher.resolve_neg()
     terms = _lib.Distillation(indices.data_ptr(), teacher.data_ptr(), _lib.ptr(labels), int(ignore_index),
                               _INDEX_BITS[indices.dtype], kind, K, int(bool(shift_labels)), temperature, soft_weight, hard_weight,
                               int(reduction == "sum"))
@@ -298,7 +301,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
     if not (0 <= int(eos_idx) < V and 0 <= int(pad_idx) < V):
         raise ValueError(f"eos_idx {eos_idx} or pad_idx {pad_idx} is not one of the {V} words")
     where = logits.device
-    scores, finished = scores.resolve_neg().contiguous(), finished.contiguous()
+    scores, finished = scores.contiguous(), finished.contiguous()
+    if scores.is_neg():
+        scores = scores.resolve_neg()
     new_scores = torch.empty(B, W, dtype=torch.float32, device=where)
     parents = torch.empty(B, W, dtype=torch.int32, device=where)
     words = torch.empty(B, W, dtype=torch.int64, device=where)
@@ -382,9 +387,10 @@ def beam_reorder(parents: torch.Tensor, states: Union[torch.Tensor, Sequence[tor
             raise ValueError(f"out[{i}] must be {tuple(s.shape)} of {s.dtype}, got {tuple(d.shape)} of {d.dtype}")
         if s.numel() == 0:
             continue
-        s = s.resolve_conj().resolve_neg()         # bytes are moved: a conjugation that only the view knows of would be lost
+        if s.is_neg() or s.dtype.is_complex:       # bytes are moved: a conjugation that only the view knows of would be lost
+            s = s.resolve_conj().resolve_neg()
         if out is not None:
-            if d.is_conj() or d.is_neg():
+            if d.is_neg() or d.is_conj():
                 raise ValueError(f"out[{i}] is a lazily conjugated or negated view")
             if any(_overlap(d, other) for other in (parents, *sources)):
                 raise ValueError(f"out[{i}] shares memory with a state or with the parents")
