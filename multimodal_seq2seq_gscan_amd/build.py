@@ -36,7 +36,7 @@ def units():
 
 # No packed fp32 instructions: some forms that the compiler makes of ordinary float code have given wrong results now and
 # then on this hardware.  The same sums of the same roundings take two instructions in place of one: the training step of
-# the compositional configuration takes 0.434 in place of 0.424 ms.  (The host pass warns that it does not know the feature.)
+# the compositional configuration takes 0.436 in place of 0.424 ms.  (The host pass warns that it does not know the feature.)
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", *NO_PACKED_FP32,
          f"-I{INCLUDE}", f"-I{CSRC}"]

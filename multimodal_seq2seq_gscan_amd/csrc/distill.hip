@@ -20,12 +20,16 @@ namespace gscan {
 
 namespace {
 constexpr int kCountBlocks = 64;
-// Up to so many rows, the launch that needs the number of live rows counts the labels itself, in every workgroup (a launch
-// less: 22.8 for 27.1 us at 5120 rows of 9 words), short rows; long ones fill the chip with workgroups, and theirs come from a launch
-// before them (4088 rows of 32000 words: 134 for 152 us).
+// Up to so many rows, the launch that needs the number of live rows counts the labels itself, in every workgroup; above, a launch
+// before it does.  Short rows (9 words of float), counted inside / before, kernels back to back and whole calls, which the host
+// binds: 1024 rows 9.4 / 10.8 and 21.5 / 23.8 us, 4096: 10.9 / 10.9 and 21.3 / 23.6, 8192: 12.9 / 11.0 and 21.3 / 23.8, 16384: 17.2 /
+// 11.1 and 21.3 / 23.6, 32768: 25.5 / 11.7 and 25.7 / 23.7: between 4096 and 16384 the one is better in a replayed graph's chain of
+// kernels, the other from the host.  Long rows, which fill the chip with workgroups: 2000 words, 256 rows 10.9 / 12.5 us, 1024:
+// 14.9 / 14.8, 2048: 20.8 / 19.2; 32000 words, 256 rows 24.0 / 25.7, 1024: 57.9 / 58.8.
 constexpr int kCountThere = 8192, kCountThereLong = 256;
-// Above so many workgroups their parts are added up by 64 workgroups before the one that finishes (rows of 100 words: 8192 rows
-// 25.6 us without and 28.5 with this launch, 16384: 32.2 and 30.5, 262144: 347 and 275).
+// Above so many workgroups their parts are added up by 64 workgroups before the one that finishes.  Without / with that launch,
+// kernels back to back: 8192 parts 54.3 / 54.4 us (131072 rows of 100 words, 16 rows a workgroup) and 32.4 / 32.6 (rows of 1030
+// words), 16384: 95.7 / 93.6 and 49.2 / 47.0, 32768: 184.0 / 177.2 and 83.7 / 77.2; 4096: 34.0 / 35.3 and 21.0 / 22.4.
 constexpr int kFinishParts = 8192;
 struct DistillArgs {
     Rows rows;
@@ -695,7 +699,9 @@ __global__ __launch_bounds__(256) void distill_group_kernel(DistillArgs a, int s
 // per row spends it on each.  262144 rows, loss and gradient / loss alone, against a wave per row: 100 words of float 94 / 53 for
 // 275 / 134 us, 200: 133 / 72 for 296 / 146, 500: 282 / 129 for 379 / 182; of bfloat16 120: 94 / 55 for 300 / 174, 500: 198 / 90
 // for 362 / 233; 32768 rows of 1000: 58 / 27 for 62 / 35.  (Against a word per lane: 9 words 32 / 17 for 55 / 37, 40 words 77 / 45
-// for 175 / 134.  Sums in 32 bits would be 3 to 10 % faster, a logarithm per row up to a third slower.)  Issue binds them up to some 200 words, the bytes beyond (500 words of float: 3.7 TB/s).
+// for 175 / 134.  Sums in 32 bits would be 3 to 10 % faster, a logarithm per row up to a third slower.)  Issue binds them up to some 200
+// words: 262144 rows of 40 words take 653 VALU instructions a wave of 4 rows, 1.00 per SIMD and four cycles, of 100 words 696 and
+// 0.88; the bytes beyond (500 words of float: 3.7 TB/s).
 constexpr int kGroupPieces = 8, kGroupLds = 48 * 1024;
 struct Group { int L, P, stride; };
 bool grouped(const gscan_rows &rows) { return cdiv(rows.V, rows.type == GSCAN_F32 ? 4 : 8) <= 16 * kGroupPieces; }
@@ -747,7 +753,7 @@ int launch_type(const DistillArgs &a, const gscan_rows &rows, hipStream_t stream
     // Registers hold a row of up to 128 KB: 8 pieces a thread while 512 threads do (32000 bfloat16 words: 104 us for 459 MB, 4.4
     // TB/s; 256 threads of 16 pieces 134 for 124, 1024 of 4 171), then 16.  Longer ones are streamed twice, the gradient past the
     // caches (4096 rows of 131072 words, 1.9 GB with a quarter of them not live: 430 us; held by 1024 threads 540).  The loss alone is
-    // one streamed pass (2000 rows of 65537 half words: 48 us).
+    // one streamed pass (2000 rows of 65537 half words: 51 us).
     if (!a.grad) {
         if (pieces <= 64 * 8) return launch_row<T, 64, 0, false>(a, stream);
         return launch_row<T, 512, 0, false>(a, stream);

@@ -454,7 +454,7 @@ __global__ __launch_bounds__(TPB) void top_row_kernel(TopArgs a) {
         s = wave_reduce(s, [](double x, double y) { return x + y; });
         if (lane == 0) sh.sum[wave] = s;
         __syncthreads();
-        if (tid == TPB - 1) {          // not of the wave that looks for the bound
+        if (tid == TPB - 1) {
             s = sh.sum[0];
             for (int w = 1; w < TPB / 64; ++w) s += sh.sum[w];
             if (a.parts) a.parts[blockIdx.x] = LsePart{s, all, 0.f};
@@ -557,7 +557,7 @@ __global__ __launch_bounds__(TPB) void top_join_kernel(TopArgs a) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) sh.keys[u * TPB + tid] = top[u];
     sh.thread_keys[tid] = max(max(top[0], top[1]), max(top[2], top[3]));
-    if (a.lse && tid >= TPB - 64) {        // the last wave: the first one looks for the bound
+    if (a.lse && tid >= TPB - 64) {        // one wave (in three workgroups of four another one than looks for the bound)
         const double total = join_lse(a.parts + (int64_t)r * a.splits, a.splits);
         if (tid == TPB - 1) a.lse[r] = (float)total;
     }
@@ -717,8 +717,9 @@ __global__ __launch_bounds__(256) void top_small_kernel(TopArgs a, int rows) {
 
 // Short rows share a wave.  262144 rows against a wave per row (a word per lane up to 64 words): 20 words of float, K = 4: 42 for
 // 86 us, 64 words: 46 for 335; 131072 rows, K = 4 / 32: 100 words of float 31 / 56 for 132 / 217, 200: 41 / 73 for 135 / 180, of
-// bfloat16 500: 58 / 104 for 162 / 213; 65536 rows of 1000: 57 / 90 for 74 / 97.  Issue binds them; 9 words are faster a word per
-// lane (25 for 43).
+// bfloat16 500: 58 / 104 for 162 / 213; 65536 rows of 1000: 57 / 90 for 74 / 97.  Issue binds them: 262144 rows of 100
+// words, K = 4, take 607 VALU instructions a wave of 4 rows, 1.04 per SIMD and four cycles (some take fewer), 131072 rows, K = 32:
+// 1049 and 0.89.  9 words are faster a word per lane (25 for 43).
 bool top_grouped(const gscan_rows &rows, int K) {
     return K <= 64 && rows.V > 16 && cdiv(rows.V, rows.type == GSCAN_F32 ? 4 : 8) <= 16 * 8;
 }

@@ -282,6 +282,8 @@ def test_sums_of_many_rows(ops, n, V):
     assert (got.cpu()[~live] == 0).all()
 
 
+# (Every size here is streamed: 512 threads hold rows of up to 32771 words of float and 65543 of 16 bits.  Those sizes, and both
+# sides of the rule, are in test_logits_instances_gpu.py.)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("V", [66000, 131075])
 def test_distillation_over_large_vocabularies(ops, dtype, V):
