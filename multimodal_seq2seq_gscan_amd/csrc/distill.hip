@@ -23,8 +23,8 @@ constexpr int kCountBlocks = 64;
 // Up to so many rows, the launch that needs the number of live rows counts the labels itself, in every workgroup; above, a launch
 // before it does.  Short rows (9 words of float), counted inside / before, kernels back to back and whole calls, which the host
 // binds: 1024 rows 9.4 / 10.8 and 21.5 / 23.8 us, 4096: 10.9 / 10.9 and 21.3 / 23.6, 8192: 12.9 / 11.0 and 21.3 / 23.8, 16384: 17.2 /
-// 11.1 and 21.3 / 23.6, 32768: 25.5 / 11.7 and 25.7 / 23.7: between 4096 and 16384 the one is better in a replayed graph's chain of
-// kernels, the other from the host.  Long rows, which fill the chip with workgroups: 2000 words, 256 rows 10.9 / 12.5 us, 1024:
+// 11.1 and 21.3 / 23.6, 32768: 25.5 / 11.7 and 25.7 / 23.7: between 4096 and 16384 rows the launch before is better in a replayed
+// graph's chain of kernels, the count inside from the host, which launches a kernel less.  Long rows, which fill the chip with workgroups: 2000 words, 256 rows 10.9 / 12.5 us, 1024:
 // 14.9 / 14.8, 2048: 20.8 / 19.2; 32000 words, 256 rows 24.0 / 25.7, 1024: 57.9 / 58.8.
 constexpr int kCountThere = 8192, kCountThereLong = 256;
 // Above so many workgroups their parts are added up by 64 workgroups before the one that finishes.  Without / with that launch,
